@@ -1914,7 +1914,7 @@ bwd64_fused_k(const float *__restrict__ g, const float *__restrict__ y,
 // 1.54 ms against 1.68 for bwd64_fused_k<.., HDX>): fetch + cut + planes 0.81 ms (4.5 GB of listed rows:
 // 5.5 TB/s), the dX phase 0.57 ms -- nearly all of it its 2.2 GB of stores, whole 128-byte lines of
 // scattered rows at 3.1 TB/s, which add to the reads instead of hiding under them -- and dW 0.16 ms, of
-// which 0.03 are its 24 MFMAs and the rest the eight accumulator flushes per tile (v_pk_fma_f32).
+// which 0.03 are its 24 MFMAs and the rest the eight accumulator flushes per tile (fp32 fma).
 // 6.7 GB in 1.54 ms = 4.35 TB/s: what is left is the memory system's mixed read/write rate on rows
 // fetched by number.
 typedef _Float16 p64h_f4 __attribute__((ext_vector_type(4)));
@@ -2119,7 +2119,7 @@ bwd64h_rows_k(const float *__restrict__ g, const float *__restrict__ y, const fl
           f32x16 acc = __builtin_amdgcn_mfma_f32_32x32x8f16(dl, xh, zero, 0, 0, 0);
           acc = __builtin_amdgcn_mfma_f32_32x32x8f16(dh, xl, acc, 0, 0, 0);
           acc = __builtin_amdgcn_mfma_f32_32x32x8f16(dh, xh, acc, 0, 0, 0);
-          // (whole-vector form: v_pk_fma_f32, two sums per instruction)
+          // (whole-vector form; one v_fma per sum: the build has packed fp32 switched off)
           if (h == 0) dw0 = __builtin_elementwise_fma(acc, unv, dw0);
           else dw1 = __builtin_elementwise_fma(acc, unv, dw1);
           __builtin_amdgcn_sched_barrier(0);
