@@ -10,6 +10,7 @@ from .encoder import StructuralEncoder, model_from_checkpoint
 from .walks import RandomWalkGenerator, CooccurrencePairSampler, estimate_pair_count
 from .trainer import (GraphSAGETrainer, BatchGenerator, StreamingBatchGenerator, Batch,
                       split_pairs_train_val, train_graphsage)
+from .norm import LayerNorm, dropout, dropout_add_layer_norm, layer_norm
 from .datafiles import load_training_data, save_training_data, load_walks
 
 __all__ = ["GraphSAGE", "SAGEConv", "create_model", "SkipGramLoss", "create_loss", "GraphCSR",
@@ -17,5 +18,6 @@ __all__ = ["GraphSAGE", "SAGEConv", "create_model", "SkipGramLoss", "create_loss
            "UniformNegativeSampler", "GraphSAGETrainer", "BatchGenerator", "Batch",
            "split_pairs_train_val", "StructuralEncoder", "model_from_checkpoint",
            "RandomWalkGenerator", "CooccurrencePairSampler", "estimate_pair_count",
-           "StreamingBatchGenerator", "train_graphsage", "load_training_data", "save_training_data", "load_walks"]
+           "StreamingBatchGenerator", "train_graphsage", "load_training_data", "save_training_data", "load_walks",
+           "LayerNorm", "dropout", "dropout_add_layer_norm", "layer_norm"]
 __version__ = "0.1.0"

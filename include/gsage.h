@@ -10,7 +10,8 @@
  * Conventions
  *   - every pointer is a DEVICE pointer unless the comment says "host";
  *   - sizes and counts are int64_t; CSR indices are int32_t (E, N < 2^31);
- *   - fp32 everywhere (the reference trains in fp32; parity bar 1e-5 relative);
+ *   - fp32 everywhere (the reference trains in fp32; parity bar 1e-5 relative), but for the layer norm
+ *     and dropout entry points, which take bf16 and fp16 tables too;
  *   - calls are asynchronous launches on `stream` (a hipStream_t passed as void*);
  *   - the library never allocates or frees device memory (callers bring the
  *     workspaces; query their sizes with the *_workspace_bytes functions);
@@ -470,6 +471,47 @@ int gsage_skipgram_bwd_rows(const float *emb, int64_t N, int64_t D, const int64_
                             const uint32_t *live_mask, const int32_t *word_prefix,
                             const int32_t *rows, const int32_t *n_rows, int64_t rows_cap, void *ws,
                             size_t ws_bytes, gsage_stream_t stream);
+
+/* ------------------------------------------- layer norm and dropout between the layers
+ * What a deeper encoder runs between its convolutions (the reference's experimental
+ * FlexibleGraphSAGE, src/model/graphsage.py:160-296, uses nn.LayerNorm, nn.Dropout and a residual sum
+ * there).  Row-major tables of fp32, bf16 or fp16 (gsage_dtype); the arithmetic is fp32, every output
+ * is rounded once.
+ *
+ *   keep(i) : the mask of GSAGE_EPI_RELU_DROPOUT: a hash of (seed, row-major element index i), kept
+ *             with probability 1 - p, 0 <= p < 1.  Never stored.  seed_dev (nullable): one int64 on
+ *             the device that takes the place of `seed`, read when the kernel runs, so that a captured
+ *             graph draws other masks on each replay.
+ *
+ * gsage_dropout: out[i] = keep(i) ? x[i] / (1 - p) : 0, whatever x[i] holds (NaN and Inf included).
+ * Its own backward: the same call on the gradient.
+ *
+ * gsage_layer_norm_fwd: with z = residual + dropout(x) (residual may be NULL, p may be 0)
+ *   y[r] = (z[r] - mean[r]) * rstd[r] * weight + bias,  rstd = 1 / sqrt(var + eps), var over the F
+ *   columns without Bessel's correction.  weight / bias [F] fp32 or of the tables' type (wdtype), each
+ *   nullable.  sum (nullable): z, rounded.  mean, rstd fp32 [M] (nullable together): for the backward.
+ *
+ * gsage_layer_norm_bwd: from grad_y (and grad_sum, nullable: the gradient of z) to
+ *   grad_x, grad_residual [M,F] and grad_weight, grad_bias [F] (wdtype), each nullable.  x, residual,
+ *   weight, p and seed as in the forward call, z and the mask are formed again.  Column sums go over
+ *   per-workgroup slabs in slab order: bitwise reproducible.  M = 0: grad_weight = grad_bias = 0.
+ *   ws: gsage_layer_norm_bwd_workspace_bytes(M, F, dtype) bytes (read only where grad_weight or
+ *   grad_bias is wanted). */
+enum gsage_dtype { GSAGE_F32 = 0, GSAGE_BF16 = 1, GSAGE_F16 = 2 };
+
+int gsage_dropout(const void *x, int64_t n, int dtype, float p, uint64_t seed,
+                  const int64_t *seed_dev, void *out, gsage_stream_t stream);
+int gsage_layer_norm_fwd(const void *x, const void *residual, const void *weight, const void *bias,
+                         int64_t M, int64_t F, int dtype, int wdtype, float eps, float p,
+                         uint64_t seed, const int64_t *seed_dev, void *y, void *sum, float *mean,
+                         float *rstd, gsage_stream_t stream);
+size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype);
+int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, const void *x,
+                         const void *residual, const void *weight, const float *mean,
+                         const float *rstd, int64_t M, int64_t F, int dtype, int wdtype, float p,
+                         uint64_t seed, const int64_t *seed_dev, void *grad_x, void *grad_residual,
+                         void *grad_weight, void *grad_bias, void *ws, size_t ws_bytes,
+                         gsage_stream_t stream);
 
 /* ----------------------------------------------------- feeder: random walks and pair windows
  * gsage_random_walks replaces RandomWalkGenerator.generate_all_walks (src/walks/generator.py:
