@@ -21,23 +21,29 @@ __device__ __forceinline__ bool dropout_keep(uint64_t seed, uint64_t idx, float 
   return u >= p;
 }
 
-// The same decisions for four consecutive elements whose indices fit 32 bits (idx + 3 < 2^32), at about
-// half the instructions: with hi = 0 the seed enters as ONE word (seed_lo ^ seed_hi), lo * C of the
-// three followers is the first product plus multiples of C (v_mul_lo_u32 is a quarter-rate
-// instruction), and u >= p on u = k 2^-24 is k >= ceil(p 2^24) on the integer k = h >> 8, i.e.
-// h >= ceil(p 2^24) << 8 (p < 1, so the threshold fits).  Bit for bit the masks of dropout_keep.
+// The hash in two parts for many elements of one upper index word: the key (once per 2^32 elements) and the draw, given
+// lo(idx) * DROPOUT_STEP (of a run's followers: the first product plus multiples of the step; v_mul_lo_u32 is a
+// quarter-rate instruction).  u >= p on u = k 2^-24 is k >= ceil(p 2^24) on the integer k = h >> 8, i.e.
+// h >= ceil(p 2^24) << 8 (p < 1, so the threshold fits): kept where dropout_draw(..) >= dropout_threshold(p), bit for
+// bit the masks of dropout_keep.
+constexpr uint32_t DROPOUT_STEP = 0x9E3779B1u;
 __device__ __forceinline__ uint32_t dropout_threshold(float p) { return ((uint32_t)ceilf(p * 16777216.0f)) << 8; }
+__device__ __forceinline__ uint32_t dropout_word(uint64_t seed, uint32_t hi) {
+  return (uint32_t)seed ^ ((uint32_t)(seed >> 32) + hi * 0x85EBCA77u);
+}
+__device__ __forceinline__ uint32_t dropout_draw(uint32_t word, uint32_t m) {
+  uint32_t h = word ^ m;
+  h ^= h >> 16;
+  h *= 0x85EBCA6Bu;
+  h ^= h >> 13;
+  h *= 0xC2B2AE35u;
+  h ^= h >> 16;
+  return h;
+}
+
+// four consecutive elements whose indices fit 32 bits (idx + 3 < 2^32), at about half the instructions
 __device__ __forceinline__ void dropout_keep4_lo(uint64_t seed, uint32_t idx, uint32_t thr, bool (&k)[4]) {
-  const uint32_t key = (uint32_t)seed ^ (uint32_t)(seed >> 32);
-  const uint32_t m0 = idx * 0x9E3779B1u;
+  const uint32_t word = dropout_word(seed, 0), m0 = idx * DROPOUT_STEP;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t h = key ^ (m0 + (uint32_t)i * 0x9E3779B1u);
-    h ^= h >> 16;
-    h *= 0x85EBCA6Bu;
-    h ^= h >> 13;
-    h *= 0xC2B2AE35u;
-    h ^= h >> 16;
-    k[i] = h >= thr;
-  }
+  for (int i = 0; i < 4; ++i) k[i] = dropout_draw(word, m0 + (uint32_t)i * DROPOUT_STEP) >= thr;
 }

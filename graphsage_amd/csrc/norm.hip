@@ -10,10 +10,86 @@
 
 namespace {
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__bf16 v) { return (float)v; }
-__device__ __forceinline__ float to_f(_Float16 v) { return (float)v; }
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
+// by value: __builtin_bit_cast straight from an element of a vector reads element 0, whatever the index
+__device__ __forceinline__ float as_f(unsigned w) { return __builtin_bit_cast(float, w); }
+__device__ __forceinline__ unsigned as_u(float f) { return __builtin_bit_cast(unsigned, f); }
+
+// ------------------------------------------------------------------ 16 bytes of a table as fp32
+// Rows start wherever they start: 16-byte accesses at element alignment, which global memory takes on this hardware
+// (the compiler emits one global_{load,store}_dwordx4 for them).
+template <typename T> struct Tab;
+template <> struct Tab<float> {
+  static constexpr int V = 4;
+  typedef u32x4 __attribute__((aligned(4), may_alias)) mem;
+  static __device__ __forceinline__ void open(u32x4 r, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = as_f(r[i]);
+  }
+  static __device__ __forceinline__ u32x4 close(const float (&f)[4]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = as_u(f[i]);
+    return r;
+  }
+};
+template <> struct Tab<__bf16> {
+  static constexpr int V = 8;
+  typedef u32x4 __attribute__((aligned(2), may_alias)) mem;
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void open(u32x4 r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = as_f(r[i] << 16);
+      f[2 * i + 1] = as_f(r[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ u32x4 close(const float (&f)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, pair{(__bf16)f[2 * i], (__bf16)f[2 * i + 1]});
+    return r;
+  }
+};
+template <> struct Tab<_Float16> {
+  static constexpr int V = 8;
+  typedef u32x4 __attribute__((aligned(2), may_alias)) mem;
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void open(u32x4 r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned word = r[i];
+      const pair h = __builtin_bit_cast(pair, word);
+      f[2 * i] = (float)h[0];
+      f[2 * i + 1] = (float)h[1];
+    }
+  }
+  static __device__ __forceinline__ u32x4 close(const float (&f)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, pair{(_Float16)f[2 * i], (_Float16)f[2 * i + 1]});
+    return r;
+  }
+};
+
+// V = 16 / sizeof(T) elements in four words, or (V = 1: rows shorter than that) one element
+template <typename T, int V> struct Raw {
+  u32x4 w;
+  __device__ __forceinline__ void zero() { w = u32x4{0u, 0u, 0u, 0u}; }
+  __device__ __forceinline__ void load(const T *p) { w = *(const typename Tab<T>::mem *)p; }
+  __device__ __forceinline__ void open(float (&f)[V]) const { Tab<T>::open(w, f); }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[V]) { *(typename Tab<T>::mem *)p = Tab<T>::close(f); }
+};
+template <typename T> struct Raw<T, 1> {
+  T w;
+  __device__ __forceinline__ void zero() { w = (T)0.f; }
+  __device__ __forceinline__ void load(const T *p) { w = *p; }
+  __device__ __forceinline__ void open(float (&f)[1]) const { f[0] = (float)w; }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
+};
+
+// ------------------------------------------------------------------ dropout
 struct Drop {              // p = 0: no mask
   float p, inv_keep;
   uint64_t seed;
@@ -21,33 +97,95 @@ struct Drop {              // p = 0: no mask
   __device__ __forceinline__ uint64_t key() const { return seed_dev ? (uint64_t)*seed_dev : seed; }
 };
 
-__device__ __forceinline__ float drop1(float v, int64_t idx, uint64_t key, const Drop &d) {
-  if (d.p <= 0.f) return v;
-  return dropout_keep(key, (uint64_t)idx, d.p) ? v * d.inv_keep : 0.f;
+// f[i] = keep(idx + i) ? f[i] / (1 - p) : 0.  The V indices share their upper word but for one vector in 2^32 / V.
+template <int V>
+__device__ __forceinline__ void drop_vec(float (&f)[V], uint64_t idx, uint64_t key, uint32_t thr, const Drop &d) {
+  const uint32_t lo = (uint32_t)idx, hi = (uint32_t)(idx >> 32);
+  if (V > 1 && lo > 0xFFFFFFFFu - (V - 1)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = dropout_keep(key, idx + i, d.p) ? f[i] * d.inv_keep : 0.f;
+    return;
+  }
+  const uint32_t k = dropout_word(key, hi), m0 = lo * DROPOUT_STEP;
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = dropout_draw(k, m0 + (uint32_t)i * DROPOUT_STEP) >= thr ? f[i] * d.inv_keep : 0.f;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_k(const T *x, int64_t n, Drop d, T *out) {
+  constexpr int V = Tab<T>::V, U = 4;
   const uint64_t key = d.key();
-  const int64_t stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride)
-    out[i] = (T)drop1(to_f(x[i]), i, key, d);
+  const uint32_t thr = dropout_threshold(d.p);
+  const int64_t nv = n / V, stride = (int64_t)gridDim.x * 256;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (; i + (U - 1) * stride < nv; i += U * stride) {
+    Raw<T, V> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u].load(x + (i + u * stride) * V);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+      r[u].open(f);
+      drop_vec<V>(f, (uint64_t)(i + u * stride) * V, key, thr, d);
+      Raw<T, V>::store(out + (i + u * stride) * V, f);
+    }
+  }
+  for (; i < nv; i += stride) {
+    Raw<T, V> r;
+    r.load(x + i * V);
+    float f[V];
+    r.open(f);
+    drop_vec<V>(f, (uint64_t)i * V, key, thr, d);
+    Raw<T, V>::store(out + i * V, f);
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n - nv * V) {      // the last n mod V elements
+    const int64_t e = nv * V + threadIdx.x;
+    out[e] = (T)(dropout_keep(key, (uint64_t)e, d.p) ? (float)x[e] * d.inv_keep : 0.f);
+  }
 }
 
-// sum over the 256 threads of a workgroup, in every thread
-__device__ __forceinline__ float block_sum(float v) {
-  __shared__ float part[4];
-  v = gs_wave_sum(v);
-  __syncthreads();
-  if (gs_lane() == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return part[0] + part[1] + part[2] + part[3];
+// ------------------------------------------------------------------ sums over the threads of a row
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+// over aligned groups of N lanes (8 .. 64), in every lane; all lanes of the wave take part
+template <int N> __device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp<0xB1>(v);                 // quad_perm: lane ^ 1
+  v += dpp<0x4E>(v);                 // quad_perm: lane ^ 2
+  v += dpp<0x141>(v);                // row_half_mirror: the other four of eight
+  if (N >= 16) v += dpp<0x140>(v);   // row_mirror: the other eight of a row
+  if (N >= 32) {                     // rows 0 <-> 1, 2 <-> 3
+    const auto r = __builtin_amdgcn_permlane16_swap(as_u(v), as_u(v), false, false);
+    v = as_f(r[0]) + as_f(r[1]);
+  }
+  if (N >= 64) {                     // the two halves of the wave
+    const auto r = __builtin_amdgcn_permlane32_swap(as_u(v), as_u(v), false, false);
+    v = as_f(r[0]) + as_f(r[1]);
+  }
+  return v;
 }
 
-__device__ __forceinline__ float load_w(const void *w, int wdtype, int64_t c) {
-  if (wdtype == GSAGE_F32) return ((const float *)w)[c];
-  if (wdtype == GSAGE_BF16) return (float)((const __bf16 *)w)[c];
-  return (float)((const _Float16 *)w)[c];
+// V weights from column c on, fp32 or of the tables' type
+template <typename T, int V> __device__ __forceinline__ void load_w(const void *w, int wdtype, int c, float (&f)[V]) {
+  if (wdtype == GSAGE_F32) {
+    const float *p = (const float *)w + c;
+    if constexpr (V == 1) f[0] = p[0];
+    else {
+#pragma unroll
+      for (int q = 0; q < V; q += 4) {
+        float o[4];
+        Raw<float, 4> r;
+        r.load(p + q);
+        r.open(o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[q + i] = o[i];
+      }
+    }
+  } else {
+    Raw<T, V> r;
+    r.load((const T *)w + c);
+    r.open(f);
+  }
 }
 __device__ __forceinline__ void store_w(void *w, int wdtype, int64_t c, float v) {
   if (wdtype == GSAGE_F32) ((float *)w)[c] = v;
@@ -58,31 +196,359 @@ __device__ __forceinline__ void store_w(void *w, int wdtype, int64_t c, float v)
 template <typename T> struct Ln {
   const T *x, *res;
   const void *w, *b;
-  int64_t M, F;
-  int wdtype;
+  int64_t M;
+  int F, wdtype;
   Drop d;
-  __device__ __forceinline__ float z(int64_t idx, uint64_t key) const {
-    const float v = drop1(to_f(x[idx]), idx, key, d);
-    return res ? to_f(res[idx]) + v : v;
+};
+
+// The columns of thread t of TPR: K vectors of V, TPR apart.  Where V does not divide F the last vector is moved back
+// to end with the row; its first `lo` elements then belong to the vector before it: both threads form and store
+// the same values, the sums count them once.
+template <int V, int TPR, int K> struct Cols {
+  int col[K], lo[K];
+  bool on[K];
+  __device__ __forceinline__ Cols(int t, int F) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int v = (t + k * TPR) * V;
+      on[k] = v < F;
+      col[k] = v < F - V ? v : F - V;
+      lo[k] = v - col[k];
+    }
+  }
+  __device__ __forceinline__ bool live(int k, int i) const { return on[k] && i >= lo[k]; }
+};
+
+// The operands of z of one row: loaded a row ahead of their use
+template <typename T, int V, int TPR, int K, bool JOIN> struct Operands {
+  Raw<T, V> x[K], r[JOIN ? K : 1];
+  __device__ __forceinline__ void load(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, bool in) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k].zero();
+      if (JOIN) r[k].zero();
+      if (in && c.on[k]) {
+        x[k].load(a.x + row * a.F + c.col[k]);
+        if (JOIN && a.res) r[k].load(a.res + row * a.F + c.col[k]);
+      }
+    }
+  }
+  __device__ __forceinline__ void z(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, uint64_t key, uint32_t thr,
+                                    float (&z)[K][V]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k].open(z[k]);
+      if (JOIN) {
+        if (a.d.p > 0.f) drop_vec<V>(z[k], (uint64_t)(row * a.F + c.col[k]), key, thr, a.d);
+        if (a.res) {
+          float q[V];
+          r[k].open(q);
+#pragma unroll
+          for (int i = 0; i < V; ++i) z[k][i] += q[i];
+        }
+      }
+    }
   }
 };
 
+// ------------------------------------------------------------------ forward
+template <typename T, int V, int TPR, int K, int NT, bool JOIN>
+__global__ void __launch_bounds__(NT) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
+  constexpr int RPB = TPR < NT ? NT / TPR : 1, NW = NT / 64;
+  static_assert(TPR <= 64 || TPR == NT, "a row takes part of a wave or the whole workgroup");
+  __shared__ float part[TPR > 64 ? 2 : 1][TPR > 64 ? NW : 1][2];
+  const int t = TPR < NT ? threadIdx.x % TPR : threadIdx.x;
+  const Cols<V, TPR, K> c(t, a.F);
+  float w[K][V], b[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) { w[k][i] = 1.f; b[k][i] = 0.f; }
+    if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
+    if (a.b && c.on[k]) load_w<T, V>(a.b, a.wdtype, c.col[k], b[k]);
+  }
+  const uint64_t key = JOIN ? a.d.key() : 0;
+  const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
+  const float inv_f = 1.0f / (float)a.F;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + (TPR < NT ? threadIdx.x / TPR : 0);
+  Operands<T, V, TPR, K, JOIN> next;
+  next.load(a, c, row, row < a.M);
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step, row += step, turn ^= 1) {
+    float z[K][V];
+    next.z(a, c, row, key, thr, z);
+    next.load(a, c, row + step, row + step < a.M);
+    float s = 0.f, q = 0.f, m, var;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += c.live(k, i) ? z[k][i] : 0.f;
+    if (TPR <= 64) {
+      m = lanes_sum<TPR <= 64 ? TPR : 64>(s) * inv_f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? z[k][i] - m : 0.f; q = fmaf(e, e, q); }
+      var = lanes_sum<TPR <= 64 ? TPR : 64>(q) * inv_f;
+    } else {
+      // each wave about its own mean, the waves' (count, mean, sum of squares) then put together:
+      // one barrier a row (the slots alternate), and no difference of large sums
+      int cnt = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int first = ((threadIdx.x & ~63) + k * TPR) * V;           // the wave's elements of this stretch
+        const int left = a.F - first;
+        cnt += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
+      }
+      const float mw = cnt ? lanes_sum<64>(s) / (float)cnt : 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? z[k][i] - mw : 0.f; q = fmaf(e, e, q); }
+      q = lanes_sum<64>(q);
+      if (gs_lane() == 0) { part[turn][threadIdx.x >> 6][0] = mw * (float)cnt; part[turn][threadIdx.x >> 6][1] = q; }
+      __syncthreads();
+      float tot = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) tot += part[turn][i][0];
+      m = tot * inv_f;
+      var = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int left = a.F - (i * 64 + k * TPR) * V;
+          n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
+        }
+        const float e = n ? part[turn][i][0] / (float)n - m : 0.f;
+        var += part[turn][i][1] + e * e * (float)n;
+      }
+      var *= inv_f;
+    }
+    const float rs = 1.0f / sqrtf(var + eps);
+    if (row < a.M) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!c.on[k]) continue;
+        if (JOIN && sum) Raw<T, V>::store(sum + row * a.F + c.col[k], z[k]);
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = fmaf((z[k][i] - m) * rs, w[k][i], b[k][i]);
+        Raw<T, V>::store(y + row * a.F + c.col[k], o);
+      }
+      if (mean && t == 0) { mean[row] = m; rstd[row] = rs; }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ backward
+// acc + v with the error carried on: a thread adds up thousands of rows
+__device__ __forceinline__ void add_carry(float &acc, float &carry, float v) {
+  const float y = v - carry, t = acc + y;
+  carry = (t - acc) - y;
+  acc = t;
+}
+
+template <typename T, int V, int TPR, int K, int NT, bool JOIN>
+__global__ void __launch_bounds__(NT) ln_bwd_k(Ln<T> a, const T *g, const T *gsum, const float *mean, const float *rstd,
+                                               T *gx, T *gres, float *ws) {
+  constexpr int RPB = TPR < NT ? NT / TPR : 1, NW = NT / 64;
+  static_assert(TPR <= 64 || TPR == NT, "a row takes part of a wave or the whole workgroup");
+  __shared__ float part[TPR > 64 ? 2 : 1][TPR > 64 ? NW : 1][2];
+  __shared__ float colsum[TPR > 64 ? 1 : NW][TPR > 64 ? 1 : 2 * TPR * K * V];
+  const int t = TPR < NT ? threadIdx.x % TPR : threadIdx.x;
+  const Cols<V, TPR, K> c(t, a.F);
+  float w[K][V], dw[K][V], db[K][V], dwc[K][V], dbc[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) { w[k][i] = 1.f; dw[k][i] = db[k][i] = dwc[k][i] = dbc[k][i] = 0.f; }
+    if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
+  }
+  const uint64_t key = JOIN ? a.d.key() : 0;
+  const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
+  const float inv_f = 1.0f / (float)a.F;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + (TPR < NT ? threadIdx.x / TPR : 0);
+  Operands<T, V, TPR, K, JOIN> next;
+  Raw<T, V> gnext[K], snext[JOIN ? K : 1];
+  float mnext = 0.f, rnext = 0.f;
+  const auto fetch = [&](int64_t r) {
+    const bool in = r < a.M;
+    next.load(a, c, r, in);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      gnext[k].zero();
+      if (JOIN) snext[k].zero();
+      if (in && c.on[k]) {
+        gnext[k].load(g + r * a.F + c.col[k]);
+        if (JOIN && gsum) snext[k].load(gsum + r * a.F + c.col[k]);
+      }
+    }
+    mnext = in ? mean[r] : 0.f;
+    rnext = in ? rstd[r] : 0.f;
+  };
+  fetch(row);
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step, row += step, turn ^= 1) {
+    float h[K][V], gv[K][V], sv[JOIN ? K : 1][V];
+    next.z(a, c, row, key, thr, h);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      gnext[k].open(gv[k]);
+      if (JOIN) snext[k].open(sv[k]);
+    }
+    const float m = mnext, rs = rnext;
+    fetch(row + step);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        h[k][i] = (h[k][i] - m) * rs;
+        add_carry(dw[k][i], dwc[k][i], gv[k][i] * h[k][i]);
+        add_carry(db[k][i], dbc[k][i], gv[k][i]);
+        gv[k][i] *= w[k][i];
+        const float e = c.live(k, i) ? gv[k][i] : 0.f;
+        s1 += e;
+        s2 = fmaf(e, h[k][i], s2);
+      }
+    if (TPR <= 64) {
+      s1 = lanes_sum<TPR <= 64 ? TPR : 64>(s1);
+      s2 = lanes_sum<TPR <= 64 ? TPR : 64>(s2);
+    } else {
+      s1 = lanes_sum<64>(s1);
+      s2 = lanes_sum<64>(s2);
+      if (gs_lane() == 0) { part[turn][threadIdx.x >> 6][0] = s1; part[turn][threadIdx.x >> 6][1] = s2; }
+      __syncthreads();
+      s1 = s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) { s1 += part[turn][i][0]; s2 += part[turn][i][1]; }
+    }
+    s1 *= inv_f;
+    s2 *= inv_f;
+    if (row < a.M) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!c.on[k]) continue;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          o[i] = rs * (gv[k][i] - s1 - h[k][i] * s2);
+          if (JOIN) o[i] += sv[k][i];
+        }
+        if (JOIN && gres) Raw<T, V>::store(gres + row * a.F + c.col[k], o);
+        if (gx) {
+          if (JOIN && a.d.p > 0.f) drop_vec<V>(o, (uint64_t)(row * a.F + c.col[k]), key, thr, a.d);
+          Raw<T, V>::store(gx + row * a.F + c.col[k], o);
+        }
+      }
+    }
+  }
+  if (!ws) return;
+  // this workgroup's column sums -> its slab
+  float *slab = ws + (int64_t)blockIdx.x * 2 * a.F;
+  if (TPR > 64) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c.live(k, i)) {
+          slab[c.col[k] + i] = dw[k][i];
+          slab[a.F + c.col[k] + i] = db[k][i];
+        }
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        for (int o = TPR; o < 64; o <<= 1) {
+          dw[k][i] += __shfl_xor(dw[k][i], o, 64);
+          db[k][i] += __shfl_xor(db[k][i], o, 64);
+        }
+        if (gs_lane() < TPR) {
+          float *p = colsum[threadIdx.x >> 6] + ((t + k * TPR) * V + i) * 2;
+          p[0] = dw[k][i];
+          p[1] = db[k][i];
+        }
+      }
+    __syncthreads();
+    if (threadIdx.x < TPR) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (c.live(k, i)) {
+            float u = 0.f, v = 0.f;
+#pragma unroll
+            for (int q = 0; q < NW; ++q) {
+              u += colsum[q][((t + k * TPR) * V + i) * 2];
+              v += colsum[q][((t + k * TPR) * V + i) * 2 + 1];
+            }
+            slab[c.col[k] + i] = u;
+            slab[a.F + c.col[k] + i] = v;
+          }
+    }
+  }
+}
+
+// The slabs' sum, in slab order per thread and in double: 16 columns of the 2 F a workgroup, 64 slabs at a time
+__global__ void __launch_bounds__(1024) ln_slabs_k(const float *ws, int slabs, int F, int wdtype, void *gw, void *gb) {
+  __shared__ double part[64][16];
+  const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+  const int s0 = threadIdx.x >> 4;
+  double v = 0.;
+  if (c < 2 * (int64_t)F)
+#pragma unroll 8
+    for (int s = s0; s < slabs; s += 64) v += (double)ws[(int64_t)s * 2 * F + c];
+  part[s0][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (threadIdx.x < 16 && c < 2 * (int64_t)F) {
+    v = 0.;
+    for (int s = 0; s < 64; ++s) v += part[s][threadIdx.x];
+    if (c < F) { if (gw) store_w(gw, wdtype, c, (float)v); }
+    else if (gb) store_w(gb, wdtype, c - F, (float)v);
+  }
+}
+
+// ------------------------------------------------------------------ rows longer than a workgroup's registers
+__device__ __forceinline__ float block_sum(float v) {      // over 1024 threads, in every thread
+  __shared__ float part[16];
+  v = lanes_sum<64>(v);
+  __syncthreads();
+  if (gs_lane() == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v += part[i];
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ float long_z(const Ln<T> &a, int64_t idx, uint64_t key) {
+  float v = (float)a.x[idx];
+  if (a.d.p > 0.f) v = dropout_keep(key, (uint64_t)idx, a.d.p) ? v * a.d.inv_keep : 0.f;
+  return a.res ? (float)a.res[idx] + v : v;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
+__global__ void __launch_bounds__(1024) ln_fwd_long_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
   const uint64_t key = a.d.key();
   const float inv_f = 1.0f / (float)a.F;
   for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
     const int64_t base = r * a.F;
     float s = 0.f, q = 0.f;
-    for (int64_t c = threadIdx.x; c < a.F; c += 256) s += a.z(base + c, key);
+    for (int c = threadIdx.x; c < a.F; c += 1024) s += long_z(a, base + c, key);
     const float m = block_sum(s) * inv_f;
-    for (int64_t c = threadIdx.x; c < a.F; c += 256) { const float t = a.z(base + c, key) - m; q += t * t; }
+    for (int c = threadIdx.x; c < a.F; c += 1024) { const float e = long_z(a, base + c, key) - m; q = fmaf(e, e, q); }
     const float rs = 1.0f / sqrtf(block_sum(q) * inv_f + eps);
-    for (int64_t c = threadIdx.x; c < a.F; c += 256) {
-      const float z = a.z(base + c, key);
-      const float h = (z - m) * rs;
-      const float w = a.w ? load_w(a.w, a.wdtype, c) : 1.f, b = a.b ? load_w(a.b, a.wdtype, c) : 0.f;
-      y[base + c] = (T)(h * w + b);
+    for (int c = threadIdx.x; c < a.F; c += 1024) {
+      const float z = long_z(a, base + c, key);
+      float w[1] = {1.f}, b[1] = {0.f};
+      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
+      if (a.b) load_w<T, 1>(a.b, a.wdtype, c, b);
+      y[base + c] = (T)fmaf((z - m) * rs, w[0], b[0]);
       if (sum) sum[base + c] = (T)z;
     }
     if (mean && threadIdx.x == 0) { mean[r] = m; rstd[r] = rs; }
@@ -90,65 +556,83 @@ __global__ void __launch_bounds__(256) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) ln_dz_k(Ln<T> a, const T *g, const T *gsum, const float *mean,
-                                               const float *rstd, T *gx, T *gres) {
+__global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const T *gsum, const float *mean,
+                                                     const float *rstd, T *gx, T *gres) {
   const uint64_t key = a.d.key();
   const float inv_f = 1.0f / (float)a.F;
   for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
     const int64_t base = r * a.F;
     const float m = mean[r], rs = rstd[r];
     float s1 = 0.f, s2 = 0.f;
-    for (int64_t c = threadIdx.x; c < a.F; c += 256) {
-      const float h = (a.z(base + c, key) - m) * rs;
-      const float t = to_f(g[base + c]) * (a.w ? load_w(a.w, a.wdtype, c) : 1.f);
-      s1 += t; s2 += t * h;
+    for (int c = threadIdx.x; c < a.F; c += 1024) {
+      const float h = (long_z(a, base + c, key) - m) * rs;
+      float w[1] = {1.f};
+      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
+      const float e = (float)g[base + c] * w[0];
+      s1 += e;
+      s2 = fmaf(e, h, s2);
     }
     s1 = block_sum(s1) * inv_f;
     s2 = block_sum(s2) * inv_f;
-    for (int64_t c = threadIdx.x; c < a.F; c += 256) {
+    for (int c = threadIdx.x; c < a.F; c += 1024) {
       const int64_t i = base + c;
-      const float h = (a.z(i, key) - m) * rs;
-      const float t = to_f(g[i]) * (a.w ? load_w(a.w, a.wdtype, c) : 1.f);
-      float dz = rs * (t - s1 - h * s2);
-      if (gsum) dz += to_f(gsum[i]);
+      const float h = (long_z(a, i, key) - m) * rs;
+      float w[1] = {1.f};
+      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
+      const float e = (float)g[i] * w[0];
+      float dz = rs * (e - s1 - h * s2);
+      if (gsum) dz += (float)gsum[i];
       if (gres) gres[i] = (T)dz;
-      if (gx) gx[i] = (T)drop1(dz, i, key, a.d);
+      if (gx) gx[i] = (T)(a.d.p <= 0.f ? dz : dropout_keep(key, (uint64_t)i, a.d.p) ? dz * a.d.inv_keep : 0.f);
     }
   }
 }
 
-// grad_w / grad_b: slab s of workgroup (column tile, s) holds the sums over its rows
 template <typename T>
-__global__ void __launch_bounds__(256) ln_dw_k(Ln<T> a, const T *g, const float *mean, const float *rstd,
-                                               float *ws) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const float *mean, const float *rstd, float *ws) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.F) return;
   const uint64_t key = a.d.key();
-  float dw = 0.f, db = 0.f;
+  float dw = 0.f, db = 0.f, dwc = 0.f, dbc = 0.f;
   for (int64_t r = blockIdx.y; r < a.M; r += gridDim.y) {
-    const float gv = to_f(g[r * a.F + c]);
-    dw += gv * ((a.z(r * a.F + c, key) - mean[r]) * rstd[r]);
-    db += gv;
+    const float gv = (float)g[r * a.F + c];
+    add_carry(dw, dwc, gv * ((long_z(a, r * a.F + c, key) - mean[r]) * rstd[r]));
+    add_carry(db, dbc, gv);
   }
   float *slab = ws + (int64_t)blockIdx.y * 2 * a.F;
   slab[c] = dw;
   slab[a.F + c] = db;
 }
 
-__global__ void __launch_bounds__(256) ln_dw_sum_k(const float *ws, int slabs, int64_t F, int wdtype, void *gw,
-                                                   void *gb) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= F) return;
-  double dw = 0., db = 0.;
-  for (int s = 0; s < slabs; ++s) {
-    dw += ws[(int64_t)s * 2 * F + c];
-    db += ws[(int64_t)s * 2 * F + F + c];
-  }
-  if (gw) store_w(gw, wdtype, c, (float)dw);
-  if (gb) store_w(gb, wdtype, c, (float)db);
+// ------------------------------------------------------------------ which kernel
+// Threads a row and vectors a thread: enough lanes that a thread holds one vector while a row fits a wave, two below
+// two waves' worth; then a workgroup a row.
+enum Form { R8, R16, R32, R64, R64x2, B256, B256x2, B512x2, B512x4, B512x8, LONG, ONE };
+Form ln_form(int64_t F, int V, bool backward) {
+  if (F < V) return ONE;
+  const int64_t nv = (F + V - 1) / V;
+  if (nv <= 8) return R8;
+  if (nv <= 16) return R16;
+  if (nv <= 32) return R32;
+  if (nv <= 64) return R64;
+  if (nv <= 128) return R64x2;
+  if (nv <= 256) return B256;
+  if (nv <= 512) return B256x2;
+  if (nv <= 1024) return B512x2;
+  // the backward holds three values and four sums an element: 16 elements a thread at most
+  if (nv <= 2048 && (V == 4 || !backward)) return B512x4;
+  if (nv <= 4096 && V == 4 && !backward) return B512x8;
+  return LONG;
 }
-
-int ln_slabs(int64_t M) { return (int)(M < 256 ? M : 256); }
+int ln_rows_per_block(Form f) {
+  return f == ONE || f == R8 ? 32 : f == R16 ? 16 : f == R32 ? 8 : f == R64 || f == R64x2 ? 4 : 1;
+}
+int ln_slabs(int64_t M, int64_t F, int V) {
+  const Form f = ln_form(F, V, true);
+  const int64_t rpb = ln_rows_per_block(f), b = (M + rpb - 1) / rpb;
+  const int64_t cap = f == B256 || f == B256x2 || f == B512x2 || f == B512x4 ? 512 : f == LONG ? 256 : 1024;
+  return (int)(b < cap ? b : cap);
+}
 
 // sizes the kernels' index arithmetic holds for: M F elements counted in int64, columns in int32
 constexpr int64_t MAX_F = 1 << 24;
@@ -157,32 +641,87 @@ constexpr int64_t MAX_N = (int64_t)1 << 40;
 bool bad_dtype(int d) { return d != GSAGE_F32 && d != GSAGE_BF16 && d != GSAGE_F16; }
 bool bad_p(float p) { return !(p >= 0.f && p < 1.f); }
 
+template <typename T, int V, int TPR, int K, int NT>
+void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
+  constexpr int RPB = TPR < NT ? NT / TPR : 1;
+  const dim3 grid(gs_grid(a.M, RPB, 256 * 2048 / NT));
+  if (a.res || a.d.p > 0.f || sum)
+    hipLaunchKernelGGL((ln_fwd_k<T, V, TPR, K, NT, true>), grid, dim3(NT), 0, st, a, eps, y, sum, mean, rstd);
+  else
+    hipLaunchKernelGGL((ln_fwd_k<T, V, TPR, K, NT, false>), grid, dim3(NT), 0, st, a, eps, y, sum, mean, rstd);
+}
+
 template <typename T>
 int ln_fwd(const void *x, const void *res, const void *w, const void *b, int64_t M, int64_t F, int wdtype, float eps,
            const Drop &d, void *y, void *sum, float *mean, float *rstd, hipStream_t st) {
-  Ln<T> a{(const T *)x, (const T *)res, w, b, M, F, wdtype, d};
-  hipLaunchKernelGGL(ln_fwd_k<T>, dim3(gs_grid(M, 1)), dim3(256), 0, st, a, eps, (T *)y, (T *)sum, mean, rstd);
+  constexpr int V = Tab<T>::V;
+  const Ln<T> a{(const T *)x, (const T *)res, w, b, M, (int)F, wdtype, d};
+#define GO(V, TPR, K, NT) ln_fwd_go<T, V, TPR, K, NT>(a, eps, (T *)y, (T *)sum, mean, rstd, st); break
+  switch (ln_form(F, V, false)) {
+    case ONE: GO(1, 8, 1, 256);
+    case R8: GO(V, 8, 1, 256);
+    case R16: GO(V, 16, 1, 256);
+    case R32: GO(V, 32, 1, 256);
+    case R64: GO(V, 64, 1, 256);
+    case R64x2: GO(V, 64, 2, 256);
+    case B256: GO(V, 256, 1, 256);
+    case B256x2: GO(V, 256, 2, 256);
+    case B512x2: GO(V, 512, 2, 512);
+    case B512x4: GO(V, 512, 4, 512);
+    case B512x8: if constexpr (V == 4) { GO(V, 512, 8, 512); } else return GSAGE_ERR_UNSUPPORTED;
+    case LONG:
+      hipLaunchKernelGGL(ln_fwd_long_k<T>, dim3(gs_grid(M, 1, 512)), dim3(1024), 0, st, a, eps, (T *)y, (T *)sum, mean, rstd);
+  }
+#undef GO
   GSAGE_CHECK_LAUNCH();
   return GSAGE_OK;
+}
+
+template <typename T, int V, int TPR, int K, int NT>
+void ln_bwd_go(const Ln<T> &a, int blocks, const T *g, const T *gsum, const float *mean, const float *rstd, T *gx, T *gres,
+               float *ws, hipStream_t st) {
+  if (a.res || a.d.p > 0.f || gsum || gres)
+    hipLaunchKernelGGL((ln_bwd_k<T, V, TPR, K, NT, true>), dim3(blocks), dim3(NT), 0, st, a, g, gsum, mean, rstd, gx, gres, ws);
+  else
+    hipLaunchKernelGGL((ln_bwd_k<T, V, TPR, K, NT, false>), dim3(blocks), dim3(NT), 0, st, a, g, gsum, mean, rstd, gx, gres, ws);
 }
 
 template <typename T>
 int ln_bwd(const void *g, const void *gsum, const void *x, const void *res, const void *w, const float *mean,
            const float *rstd, int64_t M, int64_t F, int wdtype, const Drop &d, void *gx, void *gres, void *gw, void *gb,
            float *ws, hipStream_t st) {
-  Ln<T> a{(const T *)x, (const T *)res, w, nullptr, M, F, wdtype, d};
-  const unsigned tiles = (unsigned)((F + 255) / 256);
-  if (M > 0 && (gx || gres)) {
-    hipLaunchKernelGGL(ln_dz_k<T>, dim3(gs_grid(M, 1)), dim3(256), 0, st, a, (const T *)g, (const T *)gsum, mean, rstd,
-                       (T *)gx, (T *)gres);
+  constexpr int V = Tab<T>::V;
+  const Ln<T> a{(const T *)x, (const T *)res, w, nullptr, M, (int)F, wdtype, d};
+  const int slabs = ln_slabs(M, F, V);
+  if (!gw && !gb) ws = nullptr;
+  if (M > 0 && (gx || gres || ws)) {
+#define GO(V, TPR, K, NT) \
+  ln_bwd_go<T, V, TPR, K, NT>(a, slabs, (const T *)g, (const T *)gsum, mean, rstd, (T *)gx, (T *)gres, ws, st); break
+    switch (ln_form(F, V, true)) {
+      case ONE: GO(1, 8, 1, 256);
+      case R8: GO(V, 8, 1, 256);
+      case R16: GO(V, 16, 1, 256);
+      case R32: GO(V, 32, 1, 256);
+      case R64: GO(V, 64, 1, 256);
+      case R64x2: GO(V, 64, 2, 256);
+      case B256: GO(V, 256, 1, 256);
+      case B256x2: GO(V, 256, 2, 256);
+      case B512x2: GO(V, 512, 2, 512);
+      case B512x4: if constexpr (V == 4) { GO(V, 512, 4, 512); } else return GSAGE_ERR_UNSUPPORTED;
+      case B512x8: return GSAGE_ERR_UNSUPPORTED;
+      case LONG:
+        if (gx || gres)
+          hipLaunchKernelGGL(ln_dz_long_k<T>, dim3(gs_grid(M, 1, 512)), dim3(1024), 0, st, a, (const T *)g, (const T *)gsum,
+                             mean, rstd, (T *)gx, (T *)gres);
+        if (ws)
+          hipLaunchKernelGGL(ln_dw_long_k<T>, dim3((unsigned)((F + 255) / 256), slabs), dim3(256), 0, st, a, (const T *)g,
+                             mean, rstd, ws);
+    }
+#undef GO
     GSAGE_CHECK_LAUNCH();
   }
-  if (gw || gb) {
-    if (M > 0) {
-      hipLaunchKernelGGL(ln_dw_k<T>, dim3(tiles, ln_slabs(M)), dim3(256), 0, st, a, (const T *)g, mean, rstd, ws);
-      GSAGE_CHECK_LAUNCH();
-    }
-    hipLaunchKernelGGL(ln_dw_sum_k, dim3(tiles), dim3(256), 0, st, ws, ln_slabs(M), F, wdtype, gw, gb);
+  if (ws) {
+    hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * F + 15) / 16)), dim3(1024), 0, st, ws, slabs, (int)F, wdtype, gw, gb);
     GSAGE_CHECK_LAUNCH();
   }
   return GSAGE_OK;
@@ -197,7 +736,7 @@ extern "C" int gsage_dropout(const void *x, int64_t n, int dtype, float p, uint6
   if (!x || !out) return GSAGE_ERR_INVALID_ARG;
   if (n > MAX_N) return GSAGE_ERR_UNSUPPORTED;
   const Drop d{p, 1.0f / (1.0f - p), seed, seed_dev};
-  const dim3 grid(gs_grid(n, 256)), block(256);
+  const dim3 grid(gs_grid(n, 256 * 16)), block(256);
   hipStream_t st = gs_stream(stream);
   if (dtype == GSAGE_F32) hipLaunchKernelGGL(dropout_k<float>, grid, block, 0, st, (const float *)x, n, d, (float *)out);
   else if (dtype == GSAGE_BF16) hipLaunchKernelGGL(dropout_k<__bf16>, grid, block, 0, st, (const __bf16 *)x, n, d, (__bf16 *)out);
@@ -223,7 +762,7 @@ extern "C" int gsage_layer_norm_fwd(const void *x, const void *residual, const v
 
 extern "C" size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype) {
   if (M < 0 || F <= 0 || F > MAX_F || bad_dtype(dtype)) return 0;
-  const size_t slabs = (size_t)ln_slabs(M);
+  const size_t slabs = (size_t)ln_slabs(M, F, dtype == GSAGE_F32 ? 4 : 8);
   return gs_align_up((slabs ? slabs : 1) * 2 * (size_t)F * sizeof(float), 256);
 }
 
