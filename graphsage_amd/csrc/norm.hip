@@ -5,6 +5,8 @@
 //   grad_residual = dz;  grad_x = dropout'(dz);  grad_w = sum_rows g h;  grad_b = sum_rows g
 //
 // Neither the mask nor z is stored: both are formed again from (seed, index) and from x and residual.
+#include <atomic>
+
 #include "gsage_common.h"
 #include "gsage_dropout.h"
 
@@ -73,20 +75,29 @@ template <> struct Tab<_Float16> {
   }
 };
 
-// V = 16 / sizeof(T) elements in four words, or (V = 1: rows shorter than that) one element
+// V = 16 / sizeof(T) elements in four words, or (V = 1: rows shorter than that) one element.
+// NT: accesses that are not to be kept in the caches
 template <typename T, int V> struct Raw {
   u32x4 w;
   __device__ __forceinline__ void zero() { w = u32x4{0u, 0u, 0u, 0u}; }
-  __device__ __forceinline__ void load(const T *p) { w = *(const typename Tab<T>::mem *)p; }
+  template <bool NT = false> __device__ __forceinline__ void load(const T *p) {
+    const auto *q = (const typename Tab<T>::mem *)p;
+    if constexpr (NT) w = __builtin_nontemporal_load(q);
+    else w = *q;
+  }
   __device__ __forceinline__ void open(float (&f)[V]) const { Tab<T>::open(w, f); }
-  static __device__ __forceinline__ void store(T *p, const float (&f)[V]) { *(typename Tab<T>::mem *)p = Tab<T>::close(f); }
+  template <bool NT = false> static __device__ __forceinline__ void store(T *p, const float (&f)[V]) {
+    auto *q = (typename Tab<T>::mem *)p;
+    if constexpr (NT) __builtin_nontemporal_store(Tab<T>::close(f), q);
+    else *q = Tab<T>::close(f);
+  }
 };
 template <typename T> struct Raw<T, 1> {
   T w;
   __device__ __forceinline__ void zero() { w = (T)0.f; }
-  __device__ __forceinline__ void load(const T *p) { w = *p; }
+  template <bool NT = false> __device__ __forceinline__ void load(const T *p) { w = *p; }
   __device__ __forceinline__ void open(float (&f)[1]) const { f[0] = (float)w; }
-  static __device__ __forceinline__ void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
+  template <bool NT = false> static __device__ __forceinline__ void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
 };
 
 // ------------------------------------------------------------------ dropout
@@ -97,46 +108,50 @@ struct Drop {              // p = 0: no mask
   __device__ __forceinline__ uint64_t key() const { return seed_dev ? (uint64_t)*seed_dev : seed; }
 };
 
-// f[i] = keep(idx + i) ? f[i] / (1 - p) : 0.  The V indices share their upper word but for one vector in 2^32 / V.
+// kept[i] = keep(idx + i).  The V indices share their upper word but for one vector in 2^32 / V.
 template <int V>
-__device__ __forceinline__ void drop_vec(float (&f)[V], uint64_t idx, uint64_t key, uint32_t thr, const Drop &d) {
+__device__ __forceinline__ void draw_vec(bool (&kept)[V], uint64_t idx, uint64_t key, uint32_t thr, float p) {
   const uint32_t lo = (uint32_t)idx, hi = (uint32_t)(idx >> 32);
   if (V > 1 && lo > 0xFFFFFFFFu - (V - 1)) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = dropout_keep(key, idx + i, d.p) ? f[i] * d.inv_keep : 0.f;
+    for (int i = 0; i < V; ++i) kept[i] = dropout_keep(key, idx + i, p);
     return;
   }
   const uint32_t k = dropout_word(key, hi), m0 = lo * DROPOUT_STEP;
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = dropout_draw(k, m0 + (uint32_t)i * DROPOUT_STEP) >= thr ? f[i] * d.inv_keep : 0.f;
+  for (int i = 0; i < V; ++i) kept[i] = dropout_draw(k, m0 + (uint32_t)i * DROPOUT_STEP) >= thr;
+}
+template <int V> __device__ __forceinline__ void drop_vec(float (&f)[V], const bool (&kept)[V], float inv_keep) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = kept[i] ? f[i] * inv_keep : 0.f;
 }
 
-template <typename T>
+template <typename T, bool NT>
 __global__ void __launch_bounds__(256) dropout_k(const T *x, int64_t n, Drop d, T *out) {
   constexpr int V = Tab<T>::V, U = 4;
   const uint64_t key = d.key();
   const uint32_t thr = dropout_threshold(d.p);
   const int64_t nv = n / V, stride = (int64_t)gridDim.x * 256;
   int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const auto put = [&](const Raw<T, V> &r, int64_t at) {
+    float f[V];
+    bool kept[V];
+    r.open(f);
+    draw_vec<V>(kept, (uint64_t)at * V, key, thr, d.p);
+    drop_vec<V>(f, kept, d.inv_keep);
+    Raw<T, V>::template store<NT>(out + at * V, f);
+  };
   for (; i + (U - 1) * stride < nv; i += U * stride) {
     Raw<T, V> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u].load(x + (i + u * stride) * V);
+    for (int u = 0; u < U; ++u) r[u].template load<NT>(x + (i + u * stride) * V);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[V];
-      r[u].open(f);
-      drop_vec<V>(f, (uint64_t)(i + u * stride) * V, key, thr, d);
-      Raw<T, V>::store(out + (i + u * stride) * V, f);
-    }
+    for (int u = 0; u < U; ++u) put(r[u], i + u * stride);
   }
   for (; i < nv; i += stride) {
     Raw<T, V> r;
-    r.load(x + i * V);
-    float f[V];
-    r.open(f);
-    drop_vec<V>(f, (uint64_t)i * V, key, thr, d);
-    Raw<T, V>::store(out + i * V, f);
+    r.template load<NT>(x + i * V);
+    put(r, i);
   }
   if (blockIdx.x == 0 && threadIdx.x < n - nv * V) {      // the last n mod V elements
     const int64_t e = nv * V + threadIdx.x;
@@ -201,26 +216,41 @@ template <typename T> struct Ln {
   Drop d;
 };
 
-// The columns of thread t of TPR: K vectors of V, TPR apart.  Where V does not divide F the last vector is moved back
-// to end with the row; its first `lo` elements then belong to the vector before it: both threads form and store
-// the same values, the sums count them once.
+// A row takes TPR lanes of a wave (RPB rows a workgroup of four waves), or (TPR = 0) a workgroup of up to MAXW waves.
+// Thread t of the row holds K vectors of V columns, a row's threads apart.  Where V does not divide F the last vector is
+// moved back to end with the row; its first `lo` elements then belong to the vector before it: both threads form and
+// store the same values, the sums count them once.
+constexpr int MAXW = 8;
 template <int V, int TPR, int K> struct Cols {
-  int col[K], lo[K];
-  bool on[K];
-  __device__ __forceinline__ Cols(int t, int F) {
+  int t, threads, col[K], lo[K];
+  bool on[K], full;
+  __device__ __forceinline__ Cols(int F) {
+    t = TPR ? threadIdx.x % (TPR ? TPR : 1) : threadIdx.x;
+    threads = TPR ? TPR : blockDim.x;
+    full = F == threads * K * V;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int v = (t + k * TPR) * V;
+      const int v = (t + k * threads) * V;
       on[k] = v < F;
       col[k] = v < F - V ? v : F - V;
       lo[k] = v - col[k];
     }
   }
   __device__ __forceinline__ bool live(int k, int i) const { return on[k] && i >= lo[k]; }
+  // live elements of wave i of a workgroup's row
+  __device__ __forceinline__ int wave_count(int i, int F) const {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int left = F - (i * 64 + k * threads) * V;
+      n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
+    }
+    return n;
+  }
 };
 
 // The operands of z of one row: loaded a row ahead of their use
-template <typename T, int V, int TPR, int K, bool JOIN> struct Operands {
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT> struct Operands {
   Raw<T, V> x[K], r[JOIN ? K : 1];
   __device__ __forceinline__ void load(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, bool in) {
 #pragma unroll
@@ -228,18 +258,21 @@ template <typename T, int V, int TPR, int K, bool JOIN> struct Operands {
       x[k].zero();
       if (JOIN) r[k].zero();
       if (in && c.on[k]) {
-        x[k].load(a.x + row * a.F + c.col[k]);
-        if (JOIN && a.res) r[k].load(a.res + row * a.F + c.col[k]);
+        x[k].template load<NT>(a.x + row * a.F + c.col[k]);
+        if (JOIN && a.res) r[k].template load<NT>(a.res + row * a.F + c.col[k]);
       }
     }
   }
   __device__ __forceinline__ void z(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, uint64_t key, uint32_t thr,
-                                    float (&z)[K][V]) const {
+                                    float (&z)[K][V], bool (&kept)[K][V]) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       x[k].open(z[k]);
       if (JOIN) {
-        if (a.d.p > 0.f) drop_vec<V>(z[k], (uint64_t)(row * a.F + c.col[k]), key, thr, a.d);
+        if (a.d.p > 0.f) {
+          draw_vec<V>(kept[k], (uint64_t)(row * a.F + c.col[k]), key, thr, a.d.p);
+          drop_vec<V>(z[k], kept[k], a.d.inv_keep);
+        }
         if (a.res) {
           float q[V];
           r[k].open(q);
@@ -252,13 +285,11 @@ template <typename T, int V, int TPR, int K, bool JOIN> struct Operands {
 };
 
 // ------------------------------------------------------------------ forward
-template <typename T, int V, int TPR, int K, int NT, bool JOIN>
-__global__ void __launch_bounds__(NT) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
-  constexpr int RPB = TPR < NT ? NT / TPR : 1, NW = NT / 64;
-  static_assert(TPR <= 64 || TPR == NT, "a row takes part of a wave or the whole workgroup");
-  __shared__ float part[TPR > 64 ? 2 : 1][TPR > 64 ? NW : 1][2];
-  const int t = TPR < NT ? threadIdx.x % TPR : threadIdx.x;
-  const Cols<V, TPR, K> c(t, a.F);
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+__global__ void __launch_bounds__(TPR ? 256 : 64 * MAXW) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
+  constexpr int RPB = TPR ? 256 / (TPR ? TPR : 1) : 1;
+  __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
+  const Cols<V, TPR, K> c(a.F);
   float w[K][V], b[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -270,109 +301,107 @@ __global__ void __launch_bounds__(NT) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum,
   const uint64_t key = JOIN ? a.d.key() : 0;
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
+  // (workgroup a row) this wave's elements, and those of the wave whose sums this lane puts together
+  const int mine = TPR ? 0 : c.wave_count(threadIdx.x >> 6, a.F), other = TPR ? 0 : c.wave_count(threadIdx.x % MAXW, a.F);
+  const float inv_mine = mine ? 1.0f / (float)mine : 0.f, inv_other = other ? 1.0f / (float)other : 0.f;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  int64_t row = (int64_t)blockIdx.x * RPB + (TPR < NT ? threadIdx.x / TPR : 0);
-  Operands<T, V, TPR, K, JOIN> next;
+  int64_t row = (int64_t)blockIdx.x * RPB + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
+  Operands<T, V, TPR, K, JOIN, NT> next;
   next.load(a, c, row, row < a.M);
   int turn = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step, row += step, turn ^= 1) {
     float z[K][V];
-    next.z(a, c, row, key, thr, z);
+    bool kept[K][V];
+    next.z(a, c, row, key, thr, z, kept);
     next.load(a, c, row + step, row + step < a.M);
     float s = 0.f, q = 0.f, m, var;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) s += c.live(k, i) ? z[k][i] : 0.f;
-    if (TPR <= 64) {
-      m = lanes_sum<TPR <= 64 ? TPR : 64>(s) * inv_f;
+    const auto total = [&]() {
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? z[k][i] - m : 0.f; q = fmaf(e, e, q); }
-      var = lanes_sum<TPR <= 64 ? TPR : 64>(q) * inv_f;
+        for (int i = 0; i < V; ++i) s += c.full || c.live(k, i) ? z[k][i] : 0.f;
+    };
+    const auto squares = [&](float about) {
+      if (c.full) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) { const float e = z[k][i] - about; q = fmaf(e, e, q); }
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? z[k][i] - about : 0.f; q = fmaf(e, e, q); }
+      }
+    };
+    total();
+    if constexpr (TPR != 0) {
+      m = lanes_sum<TPR>(s) * inv_f;
+      squares(m);
+      var = lanes_sum<TPR>(q) * inv_f;
     } else {
-      // each wave about its own mean, the waves' (count, mean, sum of squares) then put together:
-      // one barrier a row (the slots alternate), and no difference of large sums
-      int cnt = 0;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int first = ((threadIdx.x & ~63) + k * TPR) * V;           // the wave's elements of this stretch
-        const int left = a.F - first;
-        cnt += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
-      }
-      const float mw = cnt ? lanes_sum<64>(s) / (float)cnt : 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? z[k][i] - mw : 0.f; q = fmaf(e, e, q); }
+      // each wave about its own mean, the waves' (sum, sum of squares about it) then put together: one barrier a row
+      // (the slots alternate), and no difference of large sums
+      const float sw = lanes_sum<64>(s);
+      squares(sw * inv_mine);
       q = lanes_sum<64>(q);
-      if (gs_lane() == 0) { part[turn][threadIdx.x >> 6][0] = mw * (float)cnt; part[turn][threadIdx.x >> 6][1] = q; }
+      float(*slot)[2] = part[turn];
+      if (gs_lane() == 0) { slot[threadIdx.x >> 6][0] = sw; slot[threadIdx.x >> 6][1] = q; }
       __syncthreads();
-      float tot = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) tot += part[turn][i][0];
-      m = tot * inv_f;
-      var = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        int n = 0;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int left = a.F - (i * 64 + k * TPR) * V;
-          n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
-        }
-        const float e = n ? part[turn][i][0] / (float)n - m : 0.f;
-        var += part[turn][i][1] + e * e * (float)n;
-      }
-      var *= inv_f;
+      // (waves that are not there have no elements; their slots hold whatever LDS held)
+      const float so = other ? slot[threadIdx.x % MAXW][0] : 0.f, qo = other ? slot[threadIdx.x % MAXW][1] : 0.f;
+      m = lanes_sum<MAXW>(so) * inv_f;
+      const float e = so * inv_other - m;
+      var = lanes_sum<MAXW>(fmaf(e * e, (float)other, qo)) * inv_f;
     }
-    const float rs = 1.0f / sqrtf(var + eps);
+    const float rs = rsqrtf(var + eps);
     if (row < a.M) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!c.on[k]) continue;
-        if (JOIN && sum) Raw<T, V>::store(sum + row * a.F + c.col[k], z[k]);
+        if (JOIN && sum) Raw<T, V>::template store<NT>(sum + row * a.F + c.col[k], z[k]);
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = fmaf((z[k][i] - m) * rs, w[k][i], b[k][i]);
-        Raw<T, V>::store(y + row * a.F + c.col[k], o);
+        Raw<T, V>::template store<NT>(y + row * a.F + c.col[k], o);
       }
-      if (mean && t == 0) { mean[row] = m; rstd[row] = rs; }
+      if (mean && c.t == 0) { mean[row] = m; rstd[row] = rs; }
     }
   }
 }
 
 // ------------------------------------------------------------------ backward
-// acc + v with the error carried on: a thread adds up thousands of rows
-__device__ __forceinline__ void add_carry(float &acc, float &carry, float v) {
-  const float y = v - carry, t = acc + y;
-  carry = (t - acc) - y;
-  acc = t;
-}
+// A thread adds up the rows of its columns in two levels, 16 rows and then the sixteens: of thousands of rows in a row
+// the fp32 sum would lose some bits.
+constexpr int FLUSH = 16;
 
-template <typename T, int V, int TPR, int K, int NT, bool JOIN>
-__global__ void __launch_bounds__(NT) ln_bwd_k(Ln<T> a, const T *g, const T *gsum, const float *mean, const float *rstd,
-                                               T *gx, T *gres, float *ws) {
-  constexpr int RPB = TPR < NT ? NT / TPR : 1, NW = NT / 64;
-  static_assert(TPR <= 64 || TPR == NT, "a row takes part of a wave or the whole workgroup");
-  __shared__ float part[TPR > 64 ? 2 : 1][TPR > 64 ? NW : 1][2];
-  __shared__ float colsum[TPR > 64 ? 1 : NW][TPR > 64 ? 1 : 2 * TPR * K * V];
-  const int t = TPR < NT ? threadIdx.x % TPR : threadIdx.x;
-  const Cols<V, TPR, K> c(t, a.F);
-  float w[K][V], dw[K][V], db[K][V], dwc[K][V], dbc[K][V];
+template <typename T> struct Grads {
+  const T *g, *gsum;
+  const float *mean, *rstd;
+  T *gx, *gres;
+  float *ws;               // slabs; NULL: no column sums wanted
+  void *gw, *gb;           // written by the kernel itself where one workgroup is the whole grid
+};
+
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+__global__ void __launch_bounds__(TPR ? 256 : 64 * MAXW) ln_bwd_k(Ln<T> a, Grads<T> d) {
+  constexpr int RPB = TPR ? 256 / (TPR ? TPR : 1) : 1;
+  __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
+  __shared__ float colsum[TPR ? 4 : 1][TPR ? 2 * TPR * K * V : 1];
+  const Cols<V, TPR, K> c(a.F);
+  float w[K][V], dw[K][V], db[K][V], dw2[K][V], db2[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) { w[k][i] = 1.f; dw[k][i] = db[k][i] = dwc[k][i] = dbc[k][i] = 0.f; }
+    for (int i = 0; i < V; ++i) { w[k][i] = 1.f; dw[k][i] = db[k][i] = dw2[k][i] = db2[k][i] = 0.f; }
     if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
   }
   const uint64_t key = JOIN ? a.d.key() : 0;
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  int64_t row = (int64_t)blockIdx.x * RPB + (TPR < NT ? threadIdx.x / TPR : 0);
-  Operands<T, V, TPR, K, JOIN> next;
+  int64_t row = (int64_t)blockIdx.x * RPB + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
+  Operands<T, V, TPR, K, JOIN, NT> next;
   Raw<T, V> gnext[K], snext[JOIN ? K : 1];
   float mnext = 0.f, rnext = 0.f;
   const auto fetch = [&](int64_t r) {
@@ -383,18 +412,29 @@ __global__ void __launch_bounds__(NT) ln_bwd_k(Ln<T> a, const T *g, const T *gsu
       gnext[k].zero();
       if (JOIN) snext[k].zero();
       if (in && c.on[k]) {
-        gnext[k].load(g + r * a.F + c.col[k]);
-        if (JOIN && gsum) snext[k].load(gsum + r * a.F + c.col[k]);
+        gnext[k].template load<NT>(d.g + r * a.F + c.col[k]);
+        if (JOIN && d.gsum) snext[k].template load<NT>(d.gsum + r * a.F + c.col[k]);
       }
     }
-    mnext = in ? mean[r] : 0.f;
-    rnext = in ? rstd[r] : 0.f;
+    mnext = in ? d.mean[r] : 0.f;
+    rnext = in ? d.rstd[r] : 0.f;
+  };
+  const auto flush = [&]() {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        dw2[k][i] += dw[k][i];
+        db2[k][i] += db[k][i];
+        dw[k][i] = db[k][i] = 0.f;
+      }
   };
   fetch(row);
   int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step, row += step, turn ^= 1) {
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step, row += step, ++turn) {
     float h[K][V], gv[K][V], sv[JOIN ? K : 1][V];
-    next.z(a, c, row, key, thr, h);
+    bool kept[K][V];
+    next.z(a, c, row, key, thr, h, kept);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       gnext[k].open(gv[k]);
@@ -402,30 +442,40 @@ __global__ void __launch_bounds__(NT) ln_bwd_k(Ln<T> a, const T *g, const T *gsu
     }
     const float m = mnext, rs = rnext;
     fetch(row + step);
+    if (turn % FLUSH == FLUSH - 1) flush();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         h[k][i] = (h[k][i] - m) * rs;
-        add_carry(dw[k][i], dwc[k][i], gv[k][i] * h[k][i]);
-        add_carry(db[k][i], dbc[k][i], gv[k][i]);
+        dw[k][i] = fmaf(gv[k][i], h[k][i], dw[k][i]);
+        db[k][i] += gv[k][i];
         gv[k][i] *= w[k][i];
-        const float e = c.live(k, i) ? gv[k][i] : 0.f;
-        s1 += e;
-        s2 = fmaf(e, h[k][i], s2);
       }
-    if (TPR <= 64) {
-      s1 = lanes_sum<TPR <= 64 ? TPR : 64>(s1);
-      s2 = lanes_sum<TPR <= 64 ? TPR : 64>(s2);
+    if (c.full) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) { s1 += gv[k][i]; s2 = fmaf(gv[k][i], h[k][i], s2); }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? gv[k][i] : 0.f; s1 += e; s2 = fmaf(e, h[k][i], s2); }
+    }
+    if constexpr (TPR != 0) {
+      s1 = lanes_sum<TPR>(s1);
+      s2 = lanes_sum<TPR>(s2);
     } else {
       s1 = lanes_sum<64>(s1);
       s2 = lanes_sum<64>(s2);
-      if (gs_lane() == 0) { part[turn][threadIdx.x >> 6][0] = s1; part[turn][threadIdx.x >> 6][1] = s2; }
+      float(*slot)[2] = part[turn & 1];
+      if (gs_lane() == 0) { slot[threadIdx.x >> 6][0] = s1; slot[threadIdx.x >> 6][1] = s2; }
       __syncthreads();
-      s1 = s2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) { s1 += part[turn][i][0]; s2 += part[turn][i][1]; }
+      const bool there = threadIdx.x % MAXW < blockDim.x >> 6;
+      s1 = lanes_sum<MAXW>(there ? slot[threadIdx.x % MAXW][0] : 0.f);
+      s2 = lanes_sum<MAXW>(there ? slot[threadIdx.x % MAXW][1] : 0.f);
     }
     s1 *= inv_f;
     s2 *= inv_f;
@@ -436,42 +486,45 @@ __global__ void __launch_bounds__(NT) ln_bwd_k(Ln<T> a, const T *g, const T *gsu
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          o[i] = rs * (gv[k][i] - s1 - h[k][i] * s2);
+          o[i] = rs * fmaf(-h[k][i], s2, gv[k][i] - s1);
           if (JOIN) o[i] += sv[k][i];
         }
-        if (JOIN && gres) Raw<T, V>::store(gres + row * a.F + c.col[k], o);
-        if (gx) {
-          if (JOIN && a.d.p > 0.f) drop_vec<V>(o, (uint64_t)(row * a.F + c.col[k]), key, thr, a.d);
-          Raw<T, V>::store(gx + row * a.F + c.col[k], o);
+        if (JOIN && d.gres) Raw<T, V>::template store<NT>(d.gres + row * a.F + c.col[k], o);
+        if (d.gx) {
+          if (JOIN && a.d.p > 0.f) drop_vec<V>(o, kept[k], a.d.inv_keep);
+          Raw<T, V>::template store<NT>(d.gx + row * a.F + c.col[k], o);
         }
       }
     }
   }
-  if (!ws) return;
-  // this workgroup's column sums -> its slab
-  float *slab = ws + (int64_t)blockIdx.x * 2 * a.F;
-  if (TPR > 64) {
+  if (!d.ws) return;
+  flush();
+  // this workgroup's column sums -> its slab, or the result
+  float *slab = d.ws + (int64_t)blockIdx.x * 2 * a.F;
+  const auto put = [&](int col, float u, float v) {
+    if (gridDim.x > 1) { slab[col] = u; slab[a.F + col] = v; return; }
+    if (d.gw) store_w(d.gw, a.wdtype, col, u);
+    if (d.gb) store_w(d.gb, a.wdtype, col, v);
+  };
+  if constexpr (TPR == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (c.live(k, i)) {
-          slab[c.col[k] + i] = dw[k][i];
-          slab[a.F + c.col[k] + i] = db[k][i];
-        }
+        if (c.live(k, i)) put(c.col[k] + i, dw2[k][i], db2[k][i]);
   } else {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         for (int o = TPR; o < 64; o <<= 1) {
-          dw[k][i] += __shfl_xor(dw[k][i], o, 64);
-          db[k][i] += __shfl_xor(db[k][i], o, 64);
+          dw2[k][i] += __shfl_xor(dw2[k][i], o, 64);
+          db2[k][i] += __shfl_xor(db2[k][i], o, 64);
         }
         if (gs_lane() < TPR) {
-          float *p = colsum[threadIdx.x >> 6] + ((t + k * TPR) * V + i) * 2;
-          p[0] = dw[k][i];
-          p[1] = db[k][i];
+          float *p = colsum[threadIdx.x >> 6] + ((c.t + k * TPR) * V + i) * 2;
+          p[0] = dw2[k][i];
+          p[1] = db2[k][i];
         }
       }
     __syncthreads();
@@ -483,12 +536,11 @@ __global__ void __launch_bounds__(NT) ln_bwd_k(Ln<T> a, const T *g, const T *gsu
           if (c.live(k, i)) {
             float u = 0.f, v = 0.f;
 #pragma unroll
-            for (int q = 0; q < NW; ++q) {
-              u += colsum[q][((t + k * TPR) * V + i) * 2];
-              v += colsum[q][((t + k * TPR) * V + i) * 2 + 1];
+            for (int q = 0; q < 4; ++q) {
+              u += colsum[q][((c.t + k * TPR) * V + i) * 2];
+              v += colsum[q][((c.t + k * TPR) * V + i) * 2 + 1];
             }
-            slab[c.col[k] + i] = u;
-            slab[a.F + c.col[k] + i] = v;
+            put(c.col[k] + i, u, v);
           }
     }
   }
@@ -588,6 +640,13 @@ __global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const 
   }
 }
 
+// acc + v with the error carried on
+__device__ __forceinline__ void add_carry(float &acc, float &carry, float v) {
+  const float y = v - carry, t = acc + y;
+  carry = (t - acc) - y;
+  acc = t;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const float *mean, const float *rstd, float *ws) {
   const int c = blockIdx.x * 256 + threadIdx.x;
@@ -605,34 +664,50 @@ __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const f
 }
 
 // ------------------------------------------------------------------ which kernel
-// Threads a row and vectors a thread: enough lanes that a thread holds one vector while a row fits a wave, two below
-// two waves' worth; then a workgroup a row.
-enum Form { R8, R16, R32, R64, R64x2, B256, B256x2, B512x2, B512x4, B512x8, LONG, ONE };
+// Lanes a row: as many as it has vectors while they fit a wave, two vectors a lane up to two waves' worth; then a
+// workgroup of as many waves as K vectors a thread need.
+enum Kind { ONE, R8, R16, R32, R64, R64x2, B1, B2, B4, B8, LONG };
+struct Form { Kind kind; int threads, rows; };      // threads of a workgroup, rows it takes at once
 Form ln_form(int64_t F, int V, bool backward) {
-  if (F < V) return ONE;
+  if (F < V) return {ONE, 256, 32};
   const int64_t nv = (F + V - 1) / V;
-  if (nv <= 8) return R8;
-  if (nv <= 16) return R16;
-  if (nv <= 32) return R32;
-  if (nv <= 64) return R64;
-  if (nv <= 128) return R64x2;
-  if (nv <= 256) return B256;
-  if (nv <= 512) return B256x2;
-  if (nv <= 1024) return B512x2;
+  const auto waves = [&](int k) { return (int)((nv + 64 * k - 1) / (64 * k)) * 64; };
+  if (nv <= 8) return {R8, 256, 32};
+  if (nv <= 16) return {R16, 256, 16};
+  if (nv <= 32) return {R32, 256, 8};
+  if (nv <= 64) return {R64, 256, 4};
+  if (nv <= 128) return {R64x2, 256, 4};
+  if (nv <= 256) return {B1, waves(1), 1};
+  if (nv <= 1024) return {B2, waves(2), 1};
   // the backward holds three values and four sums an element: 16 elements a thread at most
-  if (nv <= 2048 && (V == 4 || !backward)) return B512x4;
-  if (nv <= 4096 && V == 4 && !backward) return B512x8;
-  return LONG;
+  if (nv <= 2048 && (V == 4 || !backward)) return {B4, waves(4), 1};
+  if (nv <= 4096 && V == 4 && !backward) return {B8, waves(8), 1};
+  return {LONG, 1024, 1};
 }
-int ln_rows_per_block(Form f) {
-  return f == ONE || f == R8 ? 32 : f == R16 ? 16 : f == R32 ? 8 : f == R64 || f == R64x2 ? 4 : 1;
+// Workgroups for M rows, at most `cap`, with the same number of turns each (but for the last)
+int ln_blocks(int64_t M, int rows, int cap) {
+  const int64_t groups = (M + rows - 1) / rows, turns = (groups + cap - 1) / cap;
+  return groups ? (int)((groups + turns - 1) / turns) : 0;
 }
-int ln_slabs(int64_t M, int64_t F, int V) {
-  const Form f = ln_form(F, V, true);
-  const int64_t rpb = ln_rows_per_block(f), b = (M + rpb - 1) / rpb;
-  const int64_t cap = f == B256 || f == B256x2 || f == B512x2 || f == B512x4 ? 512 : f == LONG ? 256 : 1024;
-  return (int)(b < cap ? b : cap);
+// Slabs of column sums a backward call writes at most: 1024 workgroups of four waves, fewer of more (their slabs are longer)
+int ln_slabs(int64_t M, const Form &f) { return ln_blocks(M, f.rows, f.rows > 1 ? 1024 : f.kind == LONG ? 256 : 131072 / f.threads); }
+
+// Workgroups of this kernel that the GPU holds at once: the rows are dealt out to these, none waits for a place
+template <auto KERNEL> int ln_resident(int threads) {
+  static std::atomic<int> known[MAXW + 1];
+  std::atomic<int> &n = known[threads / 64];
+  int blocks = n.load(std::memory_order_relaxed);
+  if (blocks == 0) {
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, KERNEL, threads, 0) != hipSuccess || blocks < 1) blocks = 1;
+    n.store(blocks, std::memory_order_relaxed);
+  }
+  return 256 * blocks;
 }
+
+// Tables too large for any cache (256 MB behind the L2s) are read and written past them: 10 M x 64 fp32 forward
+// 1.09 -> 1.03 ms, backward 1.55 -> 1.51, joined 1.86 -> 1.68 and 3.00 -> 2.89 ms; a 15 MB table loses that way (7.1 ->
+// 11.8 us), for the caches serve it.
+bool streams(int64_t n, size_t size) { return n * (int64_t)size >= ((int64_t)256 << 20); }
 
 // sizes the kernels' index arithmetic holds for: M F elements counted in int64, columns in int32
 constexpr int64_t MAX_F = 1 << 24;
@@ -641,14 +716,17 @@ constexpr int64_t MAX_N = (int64_t)1 << 40;
 bool bad_dtype(int d) { return d != GSAGE_F32 && d != GSAGE_BF16 && d != GSAGE_F16; }
 bool bad_p(float p) { return !(p >= 0.f && p < 1.f); }
 
-template <typename T, int V, int TPR, int K, int NT>
-void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
-  constexpr int RPB = TPR < NT ? NT / TPR : 1;
-  const dim3 grid(gs_grid(a.M, RPB, 256 * 2048 / NT));
-  if (a.res || a.d.p > 0.f || sum)
-    hipLaunchKernelGGL((ln_fwd_k<T, V, TPR, K, NT, true>), grid, dim3(NT), 0, st, a, eps, y, sum, mean, rstd);
-  else
-    hipLaunchKernelGGL((ln_fwd_k<T, V, TPR, K, NT, false>), grid, dim3(NT), 0, st, a, eps, y, sum, mean, rstd);
+template <typename T, int V, int TPR, int K>
+void ln_fwd_go(const Ln<T> &a, const Form &f, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
+  const dim3 block(f.threads);
+  const bool join = a.res || a.d.p > 0.f || sum, nt = streams(a.M * a.F, sizeof(T));
+#define GO(JOIN, NT)                                                                          \
+  hipLaunchKernelGGL((ln_fwd_k<T, V, TPR, K, JOIN, NT>),                                      \
+                     dim3(ln_blocks(a.M, f.rows, ln_resident<ln_fwd_k<T, V, TPR, K, JOIN, NT>>(f.threads))), block, 0, st, \
+                     a, eps, y, sum, mean, rstd)
+  if (join) { if (nt) GO(true, true); else GO(true, false); }
+  else { if (nt) GO(false, true); else GO(false, false); }
+#undef GO
 }
 
 template <typename T>
@@ -656,19 +734,19 @@ int ln_fwd(const void *x, const void *res, const void *w, const void *b, int64_t
            const Drop &d, void *y, void *sum, float *mean, float *rstd, hipStream_t st) {
   constexpr int V = Tab<T>::V;
   const Ln<T> a{(const T *)x, (const T *)res, w, b, M, (int)F, wdtype, d};
-#define GO(V, TPR, K, NT) ln_fwd_go<T, V, TPR, K, NT>(a, eps, (T *)y, (T *)sum, mean, rstd, st); break
-  switch (ln_form(F, V, false)) {
-    case ONE: GO(1, 8, 1, 256);
-    case R8: GO(V, 8, 1, 256);
-    case R16: GO(V, 16, 1, 256);
-    case R32: GO(V, 32, 1, 256);
-    case R64: GO(V, 64, 1, 256);
-    case R64x2: GO(V, 64, 2, 256);
-    case B256: GO(V, 256, 1, 256);
-    case B256x2: GO(V, 256, 2, 256);
-    case B512x2: GO(V, 512, 2, 512);
-    case B512x4: GO(V, 512, 4, 512);
-    case B512x8: if constexpr (V == 4) { GO(V, 512, 8, 512); } else return GSAGE_ERR_UNSUPPORTED;
+  const Form f = ln_form(F, V, false);
+#define GO(V, TPR, K) ln_fwd_go<T, V, TPR, K>(a, f, eps, (T *)y, (T *)sum, mean, rstd, st); break
+  switch (f.kind) {
+    case ONE: GO(1, 8, 1);
+    case R8: GO(V, 8, 1);
+    case R16: GO(V, 16, 1);
+    case R32: GO(V, 32, 1);
+    case R64: GO(V, 64, 1);
+    case R64x2: GO(V, 64, 2);
+    case B1: GO(V, 0, 1);
+    case B2: GO(V, 0, 2);
+    case B4: GO(V, 0, 4);
+    case B8: if constexpr (V == 4) { GO(V, 0, 8); } else return GSAGE_ERR_UNSUPPORTED;
     case LONG:
       hipLaunchKernelGGL(ln_fwd_long_k<T>, dim3(gs_grid(M, 1, 512)), dim3(1024), 0, st, a, eps, (T *)y, (T *)sum, mean, rstd);
   }
@@ -677,38 +755,47 @@ int ln_fwd(const void *x, const void *res, const void *w, const void *b, int64_t
   return GSAGE_OK;
 }
 
-template <typename T, int V, int TPR, int K, int NT>
-void ln_bwd_go(const Ln<T> &a, int blocks, const T *g, const T *gsum, const float *mean, const float *rstd, T *gx, T *gres,
-               float *ws, hipStream_t st) {
-  if (a.res || a.d.p > 0.f || gsum || gres)
-    hipLaunchKernelGGL((ln_bwd_k<T, V, TPR, K, NT, true>), dim3(blocks), dim3(NT), 0, st, a, g, gsum, mean, rstd, gx, gres, ws);
-  else
-    hipLaunchKernelGGL((ln_bwd_k<T, V, TPR, K, NT, false>), dim3(blocks), dim3(NT), 0, st, a, g, gsum, mean, rstd, gx, gres, ws);
+// -> the workgroups launched: as many slabs of column sums
+template <typename T, int V, int TPR, int K>
+int ln_bwd_go(const Ln<T> &a, const Form &f, const Grads<T> &d, hipStream_t st) {
+  const dim3 block(f.threads);
+  int slabs = ln_slabs(a.M, f);
+  const bool join = a.res || a.d.p > 0.f || d.gsum || d.gres, nt = streams(a.M * a.F, sizeof(T));
+#define GO(JOIN, NT)                                                                        \
+  {                                                                                         \
+    const int most = ln_resident<ln_bwd_k<T, V, TPR, K, JOIN, NT>>(f.threads);               \
+    if (most < slabs) slabs = ln_blocks(a.M, f.rows, most);                                  \
+    hipLaunchKernelGGL((ln_bwd_k<T, V, TPR, K, JOIN, NT>), dim3(slabs), block, 0, st, a, d); \
+  }
+  if (join) { if (nt) GO(true, true) else GO(true, false) }
+  else { if (nt) GO(false, true) else GO(false, false) }
+#undef GO
+  return slabs;
 }
 
 template <typename T>
 int ln_bwd(const void *g, const void *gsum, const void *x, const void *res, const void *w, const float *mean,
-           const float *rstd, int64_t M, int64_t F, int wdtype, const Drop &d, void *gx, void *gres, void *gw, void *gb,
+           const float *rstd, int64_t M, int64_t F, int wdtype, const Drop &drop, void *gx, void *gres, void *gw, void *gb,
            float *ws, hipStream_t st) {
   constexpr int V = Tab<T>::V;
-  const Ln<T> a{(const T *)x, (const T *)res, w, nullptr, M, (int)F, wdtype, d};
-  const int slabs = ln_slabs(M, F, V);
+  const Ln<T> a{(const T *)x, (const T *)res, w, nullptr, M, (int)F, wdtype, drop};
   if (!gw && !gb) ws = nullptr;
+  const Grads<T> d{(const T *)g, (const T *)gsum, mean, rstd, (T *)gx, (T *)gres, ws, gw, gb};
+  const Form f = ln_form(F, V, true);
+  int slabs = ln_slabs(M, f);
   if (M > 0 && (gx || gres || ws)) {
-#define GO(V, TPR, K, NT) \
-  ln_bwd_go<T, V, TPR, K, NT>(a, slabs, (const T *)g, (const T *)gsum, mean, rstd, (T *)gx, (T *)gres, ws, st); break
-    switch (ln_form(F, V, true)) {
-      case ONE: GO(1, 8, 1, 256);
-      case R8: GO(V, 8, 1, 256);
-      case R16: GO(V, 16, 1, 256);
-      case R32: GO(V, 32, 1, 256);
-      case R64: GO(V, 64, 1, 256);
-      case R64x2: GO(V, 64, 2, 256);
-      case B256: GO(V, 256, 1, 256);
-      case B256x2: GO(V, 256, 2, 256);
-      case B512x2: GO(V, 512, 2, 512);
-      case B512x4: if constexpr (V == 4) { GO(V, 512, 4, 512); } else return GSAGE_ERR_UNSUPPORTED;
-      case B512x8: return GSAGE_ERR_UNSUPPORTED;
+#define GO(V, TPR, K) slabs = ln_bwd_go<T, V, TPR, K>(a, f, d, st); break
+    switch (f.kind) {
+      case ONE: GO(1, 8, 1);
+      case R8: GO(V, 8, 1);
+      case R16: GO(V, 16, 1);
+      case R32: GO(V, 32, 1);
+      case R64: GO(V, 64, 1);
+      case R64x2: GO(V, 64, 2);
+      case B1: GO(V, 0, 1);
+      case B2: GO(V, 0, 2);
+      case B4: if constexpr (V == 4) { GO(V, 0, 4); } else return GSAGE_ERR_UNSUPPORTED;
+      case B8: return GSAGE_ERR_UNSUPPORTED;
       case LONG:
         if (gx || gres)
           hipLaunchKernelGGL(ln_dz_long_k<T>, dim3(gs_grid(M, 1, 512)), dim3(1024), 0, st, a, (const T *)g, (const T *)gsum,
@@ -720,11 +807,17 @@ int ln_bwd(const void *g, const void *gsum, const void *x, const void *res, cons
 #undef GO
     GSAGE_CHECK_LAUNCH();
   }
-  if (ws) {
+  if (ws && (slabs != 1 || f.kind == LONG)) {
     hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * F + 15) / 16)), dim3(1024), 0, st, ws, slabs, (int)F, wdtype, gw, gb);
     GSAGE_CHECK_LAUNCH();
   }
   return GSAGE_OK;
+}
+
+template <typename T> void dropout_go(const void *x, int64_t n, const Drop &d, void *out, hipStream_t st) {
+  const dim3 grid(gs_grid(n, 256 * 16)), block(256);
+  if (streams(n, sizeof(T))) hipLaunchKernelGGL((dropout_k<T, true>), grid, block, 0, st, (const T *)x, n, d, (T *)out);
+  else hipLaunchKernelGGL((dropout_k<T, false>), grid, block, 0, st, (const T *)x, n, d, (T *)out);
 }
 
 }  // namespace
@@ -736,11 +829,10 @@ extern "C" int gsage_dropout(const void *x, int64_t n, int dtype, float p, uint6
   if (!x || !out) return GSAGE_ERR_INVALID_ARG;
   if (n > MAX_N) return GSAGE_ERR_UNSUPPORTED;
   const Drop d{p, 1.0f / (1.0f - p), seed, seed_dev};
-  const dim3 grid(gs_grid(n, 256 * 16)), block(256);
   hipStream_t st = gs_stream(stream);
-  if (dtype == GSAGE_F32) hipLaunchKernelGGL(dropout_k<float>, grid, block, 0, st, (const float *)x, n, d, (float *)out);
-  else if (dtype == GSAGE_BF16) hipLaunchKernelGGL(dropout_k<__bf16>, grid, block, 0, st, (const __bf16 *)x, n, d, (__bf16 *)out);
-  else hipLaunchKernelGGL(dropout_k<_Float16>, grid, block, 0, st, (const _Float16 *)x, n, d, (_Float16 *)out);
+  if (dtype == GSAGE_F32) dropout_go<float>(x, n, d, out, st);
+  else if (dtype == GSAGE_BF16) dropout_go<__bf16>(x, n, d, out, st);
+  else dropout_go<_Float16>(x, n, d, out, st);
   GSAGE_CHECK_LAUNCH();
   return GSAGE_OK;
 }
@@ -762,7 +854,7 @@ extern "C" int gsage_layer_norm_fwd(const void *x, const void *residual, const v
 
 extern "C" size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype) {
   if (M < 0 || F <= 0 || F > MAX_F || bad_dtype(dtype)) return 0;
-  const size_t slabs = (size_t)ln_slabs(M, F, dtype == GSAGE_F32 ? 4 : 8);
+  const size_t slabs = (size_t)ln_slabs(M, ln_form(F, dtype == GSAGE_F32 ? 4 : 8, true));
   return gs_align_up((slabs ? slabs : 1) * 2 * (size_t)F * sizeof(float), 256);
 }
 
