@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(TPR ? 256 : 64 * MAXW) ln_fwd_k(Ln<T> a, float
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
   // (workgroup a row) this wave's elements, and those of the wave whose sums this lane puts together
-  const int mine = TPR ? 0 : c.wave_count(threadIdx.x >> 6, a.F), other = TPR ? 0 : c.wave_count(threadIdx.x % MAXW, a.F);
+  const int mine = TPR ? 0 : c.wave_count(threadIdx.x >> 6, a.F), 
+            other = TPR || threadIdx.x % MAXW >= blockDim.x >> 6 ? 0 : c.wave_count(threadIdx.x % MAXW, a.F);
   const float inv_mine = mine ? 1.0f / (float)mine : 0.f, inv_other = other ? 1.0f / (float)other : 0.f;
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
