@@ -1,0 +1,89 @@
+// Layer norm and dropout, host side: what norm.hip (the C entries) hands to the kernels of one type of table, and which
+// kernel a width takes.
+#pragma once
+#include "gsage_common.h"
+
+struct NormDrop {          // p = 0: no mask
+  float p, inv_keep;
+  uint64_t seed;
+  const int64_t *seed_dev;
+};
+
+struct NormFwd {
+  const void *x, *res, *w, *b;
+  int64_t M, F;
+  int wdtype;
+  float eps;
+  NormDrop d;
+  void *y, *sum;
+  float *mean, *rstd;
+};
+
+struct NormBwd {
+  const void *g, *gsum, *x, *res, *w;
+  const float *mean, *rstd;
+  int64_t M, F;
+  int wdtype;
+  NormDrop d;
+  void *gx, *gres, *gw, *gb;
+  float *ws;
+};
+
+// Which kernel a row takes: K vectors of 16 bytes (V elements each) in each of R lanes of a wave, or of `row` threads of a
+// workgroup (B); NORM_ONE: rows shorter than a vector, an element a lane.  A row's sums and addresses cost its threads the
+// same whatever they hold, so a row takes the fewest lanes that need no more than three vectors each, which also leaves
+// few of them idle (fp16, 126 MB tables, forward + backward with residual and dropout: 264 columns in 16 lanes x 3 run at
+// 4.6 and 4.0 TB/s, in 64 x 1 at 3.5 and 3.6; 1544 columns as a workgroup of 193 threads x 1 4.0, 97 x 2 4.2).  Two or
+// four waves a row rather than three or five: eight fit a compute unit.  Large tables of whole cache lines without
+// residual or dropout stream best where neighbouring lanes hold neighbouring vectors (`stream`: 10 M x 64 fp32 forward
+// 0.94 ms at 16 lanes x 1, 0.99 at 8 x 2; backward 1.41 and 1.58).
+enum NormKind { NORM_ONE, NORM_R4, NORM_R8, NORM_R8x2, NORM_R8x3, NORM_R16, NORM_R16x2, NORM_R16x3, NORM_R32, NORM_R32x2,
+                NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_B8, NORM_LONG };
+struct NormForm { NormKind kind; int row; };      // threads of a row
+static inline NormForm norm_form(int64_t F, int V, bool stream) {
+  if (F < V) return {NORM_ONE, 8};
+  const int64_t nv = (F + V - 1) / V;
+  const auto waves = [&](int k) { return (int)((nv + 64 * k - 1) / (64 * k)) * 64; };
+  if (nv <= 4) return {NORM_R4, 4};
+  if (nv <= 8) return {NORM_R8, 8};
+  if (stream && nv == 16) return {NORM_R16, 16};
+  if (stream && nv == 32) return {NORM_R32, 32};
+  if (stream && nv == 64) return {NORM_R64, 64};
+  if (nv <= 16) return {NORM_R8x2, 8};
+  if (nv <= 24) return {NORM_R8x3, 8};
+  if (nv <= 32) return {NORM_R16x2, 16};
+  if (nv <= 48) return {NORM_R16x3, 16};
+  if (nv <= 64) return {NORM_R32x2, 32};
+  if (nv <= 96) return {NORM_R32x3, 32};
+  if (nv <= 128) return {NORM_R64x2, 64};
+  if (nv <= 192) return {NORM_R64x3, 64};
+  if (nv <= 256) return {NORM_B2, 128};
+  if (nv <= 384) return {NORM_B3, 128};
+  if (nv <= 512) return {NORM_B2, 256};
+  if (nv <= 768) return {NORM_B3, waves(3)};
+  if (nv <= 1024) return {NORM_B2, waves(2)};
+  if (nv <= 2048) return {NORM_B4, waves(4)};
+  if (nv <= 4096 && V == 4) return {NORM_B8, waves(8)};
+  return {NORM_LONG, 1024};
+}
+
+// Workgroups for M rows, `rows` at once each, at most `cap`, with the same number of turns each (but for the last)
+static inline int norm_blocks(int64_t M, int rows, int cap) {
+  const int64_t groups = (M + rows - 1) / rows, turns = (groups + cap - 1) / cap;
+  return groups ? (int)((groups + turns - 1) / turns) : 0;
+}
+// Slabs of column sums a backward call writes at most
+static inline int norm_max_slabs(int64_t M, int64_t F) {
+  const int64_t cap = F <= 512 ? 1024 : F <= 8192 ? 512 : 256;
+  return (int)(M < cap ? M : cap);
+}
+
+int norm_dropout_f32(const void *x, int64_t n, const NormDrop &d, void *out, hipStream_t st);
+int norm_dropout_bf16(const void *x, int64_t n, const NormDrop &d, void *out, hipStream_t st);
+int norm_dropout_f16(const void *x, int64_t n, const NormDrop &d, void *out, hipStream_t st);
+int norm_fwd_f32(const NormFwd &n, hipStream_t st);
+int norm_fwd_bf16(const NormFwd &n, hipStream_t st);
+int norm_fwd_f16(const NormFwd &n, hipStream_t st);
+int norm_bwd_f32(const NormBwd &n, hipStream_t st);
+int norm_bwd_bf16(const NormBwd &n, hipStream_t st);
+int norm_bwd_f16(const NormBwd &n, hipStream_t st);

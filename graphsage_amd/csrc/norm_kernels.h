@@ -1,0 +1,814 @@
+// Kernels and launches of layer norm and dropout for one type of table: included by norm_f32.hip, norm_bf16.hip and
+// norm_f16.hip, which are compiled side by side.
+//
+//   z = residual + dropout(x);  y = (z - mean) rstd w + b
+//   a = g w;  h = (z - mean) rstd;  dz = rstd (a - mean(a) - h mean(a h)) + grad_sum
+//   grad_residual = dz;  grad_x = dropout'(dz);  grad_w = sum_rows g h;  grad_b = sum_rows g
+//
+// Neither the mask nor z is stored: both are formed again from (seed, index) and from x and residual.  A row is read
+// once: it lies in the registers of the threads that share it while its sums are taken.
+#pragma once
+#include <atomic>
+
+#include "gsage_common.h"
+#include "gsage_dropout.h"
+#include "norm.h"
+
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// by value: __builtin_bit_cast straight from an element of a vector reads element 0, whatever the index
+__device__ __forceinline__ float as_f(unsigned w) { return __builtin_bit_cast(float, w); }
+__device__ __forceinline__ unsigned as_u(float f) { return __builtin_bit_cast(unsigned, f); }
+
+// ------------------------------------------------------------------ 16 bytes of a table as fp32
+// Rows start wherever they start: 16-byte accesses at element alignment, which global memory takes on this hardware
+// (the compiler emits one global_{load,store}_dwordx4 for them).
+template <typename T> struct Tab;
+template <> struct Tab<float> {
+  static constexpr int V = 4;
+  typedef u32x4 __attribute__((aligned(4), may_alias)) mem;
+  static __device__ __forceinline__ void open(u32x4 r, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = as_f(r[i]);
+  }
+  static __device__ __forceinline__ u32x4 close(const float (&f)[4]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = as_u(f[i]);
+    return r;
+  }
+};
+template <> struct Tab<__bf16> {
+  static constexpr int V = 8;
+  typedef u32x4 __attribute__((aligned(2), may_alias)) mem;
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void open(u32x4 r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = as_f(r[i] << 16);
+      f[2 * i + 1] = as_f(r[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ u32x4 close(const float (&f)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, pair{(__bf16)f[2 * i], (__bf16)f[2 * i + 1]});
+    return r;
+  }
+};
+template <> struct Tab<_Float16> {
+  static constexpr int V = 8;
+  typedef u32x4 __attribute__((aligned(2), may_alias)) mem;
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void open(u32x4 r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned word = r[i];
+      const pair h = __builtin_bit_cast(pair, word);
+      f[2 * i] = (float)h[0];
+      f[2 * i + 1] = (float)h[1];
+    }
+  }
+  static __device__ __forceinline__ u32x4 close(const float (&f)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, pair{(_Float16)f[2 * i], (_Float16)f[2 * i + 1]});
+    return r;
+  }
+};
+
+// V = 16 / sizeof(T) elements in four words, or (V = 1: rows shorter than that) one element.
+// NT: accesses that are not to be kept in the caches
+template <typename T, int V> struct Raw {
+  u32x4 w;
+  __device__ __forceinline__ void zero() { w = u32x4{0u, 0u, 0u, 0u}; }
+  template <bool NT = false> __device__ __forceinline__ void load(const T *p) {
+    const auto *q = (const typename Tab<T>::mem *)p;
+    if constexpr (NT) w = __builtin_nontemporal_load(q);
+    else w = *q;
+  }
+  __device__ __forceinline__ void open(float (&f)[V]) const { Tab<T>::open(w, f); }
+  template <bool NT = false> static __device__ __forceinline__ void store(T *p, const float (&f)[V]) {
+    auto *q = (typename Tab<T>::mem *)p;
+    if constexpr (NT) __builtin_nontemporal_store(Tab<T>::close(f), q);
+    else *q = Tab<T>::close(f);
+  }
+};
+template <typename T> struct Raw<T, 1> {
+  T w;
+  __device__ __forceinline__ void zero() { w = (T)0.f; }
+  template <bool NT = false> __device__ __forceinline__ void load(const T *p) { w = *p; }
+  __device__ __forceinline__ void open(float (&f)[1]) const { f[0] = (float)w; }
+  template <bool NT = false> static __device__ __forceinline__ void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
+};
+
+// ------------------------------------------------------------------ dropout
+__device__ __forceinline__ uint64_t drop_key(const NormDrop &d) { return d.seed_dev ? (uint64_t)*d.seed_dev : d.seed; }
+
+// kept[i] = keep(idx + i).  The V indices share their upper word but for one vector in 2^32 / V.
+template <int V>
+__device__ __forceinline__ void draw_vec(bool (&kept)[V], uint64_t idx, uint64_t key, uint32_t thr, float p) {
+  const uint32_t lo = (uint32_t)idx, hi = (uint32_t)(idx >> 32);
+  if (V > 1 && lo > 0xFFFFFFFFu - (V - 1)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) kept[i] = dropout_keep(key, idx + i, p);
+    return;
+  }
+  const uint32_t k = dropout_word(key, hi), m0 = lo * DROPOUT_STEP;
+#pragma unroll
+  for (int i = 0; i < V; ++i) kept[i] = dropout_draw(k, m0 + (uint32_t)i * DROPOUT_STEP) >= thr;
+}
+template <int V> __device__ __forceinline__ void drop_vec(float (&f)[V], const bool (&kept)[V], float inv_keep) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = kept[i] ? f[i] * inv_keep : 0.f;
+}
+
+template <typename T, bool NT>
+__global__ void __launch_bounds__(256) dropout_k(const T *x, int64_t n, NormDrop d, T *out) {
+  constexpr int V = Tab<T>::V, U = 4;
+  const uint64_t key = drop_key(d);
+  const uint32_t thr = dropout_threshold(d.p);
+  const int64_t nv = n / V, stride = (int64_t)gridDim.x * 256;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const auto put = [&](const Raw<T, V> &r, int64_t at) {
+    float f[V];
+    bool kept[V];
+    r.open(f);
+    draw_vec<V>(kept, (uint64_t)at * V, key, thr, d.p);
+    drop_vec<V>(f, kept, d.inv_keep);
+    Raw<T, V>::template store<NT>(out + at * V, f);
+  };
+  for (; i + (U - 1) * stride < nv; i += U * stride) {
+    Raw<T, V> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u].template load<NT>(x + (i + u * stride) * V);
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(r[u], i + u * stride);
+  }
+  for (; i < nv; i += stride) {
+    Raw<T, V> r;
+    r.template load<NT>(x + i * V);
+    put(r, i);
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n - nv * V) {      // the last n mod V elements
+    const int64_t e = nv * V + threadIdx.x;
+    out[e] = (T)(dropout_keep(key, (uint64_t)e, d.p) ? (float)x[e] * d.inv_keep : 0.f);
+  }
+}
+
+// ------------------------------------------------------------------ sums over the threads of a row
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+// over aligned groups of N lanes (4 .. 64), in every lane; all lanes of the wave take part
+template <int N> __device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp<0xB1>(v);                 // quad_perm: lane ^ 1
+  v += dpp<0x4E>(v);                 // quad_perm: lane ^ 2
+  if (N >= 8) v += dpp<0x141>(v);    // row_half_mirror: the other four of eight
+  if (N >= 16) v += dpp<0x140>(v);   // row_mirror: the other eight of a row
+  if (N >= 32) {                     // rows 0 <-> 1, 2 <-> 3
+    const auto r = __builtin_amdgcn_permlane16_swap(as_u(v), as_u(v), false, false);
+    v = as_f(r[0]) + as_f(r[1]);
+  }
+  if (N >= 64) {                     // the two halves of the wave
+    const auto r = __builtin_amdgcn_permlane32_swap(as_u(v), as_u(v), false, false);
+    v = as_f(r[0]) + as_f(r[1]);
+  }
+  return v;
+}
+
+// V weights from column c on, fp32 or of the tables' type
+template <typename T, int V> __device__ __forceinline__ void load_w(const void *w, int wdtype, int c, float (&f)[V]) {
+  if (wdtype == GSAGE_F32) {
+    const float *p = (const float *)w + c;
+    if constexpr (V == 1) f[0] = p[0];
+    else {
+#pragma unroll
+      for (int q = 0; q < V; q += 4) {
+        float o[4];
+        Raw<float, 4> r;
+        r.load(p + q);
+        r.open(o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[q + i] = o[i];
+      }
+    }
+  } else {
+    Raw<T, V> r;
+    r.load((const T *)w + c);
+    r.open(f);
+  }
+}
+__device__ __forceinline__ void store_w(void *w, int wdtype, int64_t c, float v) {
+  if (wdtype == GSAGE_F32) ((float *)w)[c] = v;
+  else if (wdtype == GSAGE_BF16) ((__bf16 *)w)[c] = (__bf16)v;
+  else ((_Float16 *)w)[c] = (_Float16)v;
+}
+
+template <typename T> struct Ln {
+  const T *x, *res;
+  const void *w, *b;
+  int64_t M;
+  int F, wdtype, row;      // row: threads of a row, where that is not the kernel's own constant
+  NormDrop d;
+};
+
+// A row takes TPR lanes of a wave, or (TPR = 0) a.row threads: up to MAXW whole waves.  A workgroup takes as many rows at
+// once as fit.  Thread t of the row holds K vectors of V columns, a row's threads apart.  A vector that would go past the
+// row's end is moved back to end with it; its first `lo` elements (all of them, where the thread has nothing left to do)
+// then belong to vectors before it: both threads form and store the same values, the sums count them once.
+constexpr int MAXW = 8;
+template <int V, int TPR, int K> struct Cols {
+  int t, threads, col[K], lo[K];
+  bool on[K], full;
+  __device__ __forceinline__ Cols(int F, int row) {
+    threads = TPR ? TPR : row;
+    t = threadIdx.x % threads;
+    full = F == threads * K * V;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int v = (t + k * threads) * V;
+      on[k] = v < F;
+      col[k] = v < F - V ? v : F - V;
+      lo[k] = v - col[k];
+    }
+  }
+  __device__ __forceinline__ bool live(int k, int i) const { return i >= lo[k]; }
+  // live elements of wave i of a row's
+  __device__ __forceinline__ int wave_count(int i, int F) const {
+    int n = 0;
+    if (i < threads >> 6)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int left = F - (i * 64 + k * threads) * V;
+        n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
+      }
+    return n;
+  }
+};
+
+// The operands of z of one row: loaded a row ahead of their use (short rows), or at it
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT> struct Operands {
+  Raw<T, V> x[K], r[JOIN ? K : 1];
+  __device__ __forceinline__ void load(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, bool in) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k].zero();
+      if (JOIN) r[k].zero();
+      if (in && c.on[k]) {
+        x[k].template load<NT>(a.x + row * a.F + c.col[k]);
+        if (JOIN && a.res) r[k].template load<NT>(a.res + row * a.F + c.col[k]);
+      }
+    }
+  }
+  __device__ __forceinline__ void z(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, uint64_t key, uint32_t thr,
+                                    float (&z)[K][V], bool (&kept)[K][V]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k].open(z[k]);
+      if (JOIN) {
+        if (a.d.p > 0.f) {
+          draw_vec<V>(kept[k], (uint64_t)(row * a.F + c.col[k]), key, thr, a.d.p);
+          drop_vec<V>(z[k], kept[k], a.d.inv_keep);
+        }
+        if (a.res) {
+          float q[V];
+          r[k].open(q);
+#pragma unroll
+          for (int i = 0; i < V; ++i) z[k][i] += q[i];
+        }
+      }
+    }
+  }
+};
+
+// Nothing of this wave is under way (vmcnt = 0).  Streaming kernels wait so before their stores and after them: reads and
+// writes then come in turns, which the memory takes better than both at once (10 M x 64 fp32 forward 0.94 against
+// 0.99 ms; joined backward 2.36 against 2.50 ms, 1 M x 256 0.87 against 0.97).
+__device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// ------------------------------------------------------------------ forward
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+__global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW, NT && K == 1 ? 8 : 1) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
+  constexpr bool AHEAD = K * V < 32;          // 32 elements a thread: no registers left for the row after
+  __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
+  const Cols<V, TPR, K> c(a.F, a.row);
+  const int rows = TPR ? 256 / (TPR ? TPR : 1) : 1, first = TPR ? threadIdx.x / (TPR ? TPR : 1) : 0;   // rows at once, this thread's
+  float w[K][V], b[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) { w[k][i] = 1.f; b[k][i] = 0.f; }
+    if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
+    if (a.b && c.on[k]) load_w<T, V>(a.b, a.wdtype, c.col[k], b[k]);
+  }
+  const uint64_t key = JOIN ? drop_key(a.d) : 0;
+  const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
+  const float inv_f = 1.0f / (float)a.F;
+  // (rows of several waves) this wave's elements, and those of the wave whose sums this lane puts together
+  const int mine = TPR ? 0 : c.wave_count(c.t >> 6, a.F), other = TPR ? 0 : c.wave_count(threadIdx.x % MAXW, a.F);
+  const float inv_mine = mine ? 1.0f / (float)mine : 0.f, inv_other = other ? 1.0f / (float)other : 0.f;
+  const int64_t step = (int64_t)gridDim.x * rows;
+  int64_t row = (int64_t)blockIdx.x * rows + first;
+  Operands<T, V, TPR, K, JOIN, NT> next;
+  if (AHEAD) next.load(a, c, row, row < a.M);
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * rows; r0 < a.M; r0 += step, row += step, turn ^= 1) {
+    float z[K][V];
+    bool kept[K][V];
+    if (!AHEAD) next.load(a, c, row, row < a.M);
+    next.z(a, c, row, key, thr, z, kept);
+    if (AHEAD) next.load(a, c, row + step, row + step < a.M);
+    float s = 0.f, q = 0.f, m, var;
+    const auto squares = [&](float about) {
+      if (c.full) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) { const float e = z[k][i] - about; q = fmaf(e, e, q); }
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? z[k][i] - about : 0.f; q = fmaf(e, e, q); }
+      }
+    };
+    // (z is zero where a thread has no column; a moved vector's first elements are not counted again)
+    if (a.F % V == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += z[k][i];
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += c.live(k, i) ? z[k][i] : 0.f;
+    }
+    if constexpr (TPR != 0) {
+      m = lanes_sum<TPR>(s) * inv_f;
+      squares(m);
+      var = lanes_sum<TPR>(q) * inv_f;
+    } else {
+      // each wave about its own mean, the waves' (sum, sum of squares about it) then put together: one barrier a row
+      // (the slots alternate), and no difference of large sums
+      const float sw = lanes_sum<64>(s);
+      squares(sw * inv_mine);
+      q = lanes_sum<64>(q);
+      float(*slot)[2] = part[turn];
+      if (gs_lane() == 0) { slot[c.t >> 6][0] = sw; slot[c.t >> 6][1] = q; }
+      __syncthreads();
+      // (waves that are not there have no elements; their slots hold whatever LDS held)
+      const float so = other ? slot[threadIdx.x % MAXW][0] : 0.f, qo = other ? slot[threadIdx.x % MAXW][1] : 0.f;
+      m = lanes_sum<MAXW>(so) * inv_f;
+      const float e = so * inv_other - m;
+      var = lanes_sum<MAXW>(fmaf(e * e, (float)other, qo)) * inv_f;
+    }
+    const float rs = rsqrtf(var + eps);
+    if constexpr (NT) settle();
+    if (row < a.M) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!c.on[k]) continue;
+        if (JOIN && sum) Raw<T, V>::template store<NT>(sum + row * a.F + c.col[k], z[k]);
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = fmaf((z[k][i] - m) * rs, w[k][i], b[k][i]);
+        Raw<T, V>::template store<NT>(y + row * a.F + c.col[k], o);
+      }
+      if (mean && c.t == 0) { mean[row] = m; rstd[row] = rs; }
+    }
+    if constexpr (NT) settle();
+  }
+}
+
+template <typename T> struct Grads {
+  const T *g, *gsum;
+  const float *mean, *rstd;
+  T *gx, *gres;
+  float *ws;               // slabs; NULL: no column sums wanted
+  void *gw, *gb;           // written by the kernel itself where one workgroup is the whole grid
+};
+
+// ------------------------------------------------------------------ backward
+// A thread's column sums: in registers for 16 rows, then added to its own words of LDS (of thousands of rows in a row an
+// fp32 sum would lose some bits, and the registers of a second level would cost occupancy).  Where there are no registers
+// for the first level either every row goes to LDS.
+constexpr int FLUSH = 16;
+
+// Workgroups of eight waves (fewer slabs than four would leave).  With 24 elements a thread and the row after in flight
+// four have the registers: rows of several waves do better so (bf16 6000 columns joined backward 205 us, without the row
+// after 215), rows within a wave with eight waves and no row ahead (fp16 257 columns 79 -> 74 us, 1200 137 -> 128).
+constexpr bool ln_bwd_ahead(int V, int TPR, int K, bool JOIN) {
+  return K * V < (TPR ? 24 : 32) && !(JOIN && K * V == 16 && V == 4);
+}
+constexpr int ln_bwd_threads(int V, int TPR, int K) { return K == 3 && V == 8 && TPR == 0 ? 256 : 64 * MAXW; }
+
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+__global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, Grads<T> d) {
+  constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
+  constexpr int A = AHEAD ? K : 1;
+  extern __shared__ float acc[];              // [2 K V][threads]: grad_w, then grad_b; a thread's words are its own
+  __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
+  constexpr int threads = ln_bwd_threads(V, TPR, K);      // (a workgroup a row may have fewer)
+  float *const mine = acc + threadIdx.x;
+  const Cols<V, TPR, K> c(a.F, a.row);
+  const int rows = TPR ? threads / (TPR ? TPR : 1) : blockDim.x / c.threads, first = threadIdx.x / c.threads;
+  float w[K][V], dw[A][V], db[A][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[k][i] = 1.f;
+      if (AHEAD) dw[k % A][i] = db[k % A][i] = 0.f;
+      mine[(k * V + i) * threads] = mine[((K + k) * V + i) * threads] = 0.f;
+    }
+    if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
+  }
+  const uint64_t key = JOIN ? drop_key(a.d) : 0;
+  const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
+  const float inv_f = 1.0f / (float)a.F;
+  const int64_t step = (int64_t)gridDim.x * rows;
+  int64_t row = (int64_t)blockIdx.x * rows + first;
+  Operands<T, V, TPR, K, JOIN, NT> next;
+  Raw<T, V> gnext[K], snext[JOIN ? K : 1];
+  float mnext = 0.f, rnext = 0.f;
+  const auto fetch = [&](int64_t r) {
+    const bool in = r < a.M;
+    next.load(a, c, r, in);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      gnext[k].zero();
+      if (JOIN) snext[k].zero();
+      if (in && c.on[k]) {
+        gnext[k].template load<NT>(d.g + r * a.F + c.col[k]);
+        if (JOIN && d.gsum) snext[k].template load<NT>(d.gsum + r * a.F + c.col[k]);
+      }
+    }
+    mnext = in ? d.mean[r] : 0.f;
+    rnext = in ? d.rstd[r] : 0.f;
+  };
+  const auto flush = [&]() {
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          mine[(k * V + i) * threads] += dw[k][i];
+          mine[((K + k) * V + i) * threads] += db[k][i];
+          dw[k][i] = db[k][i] = 0.f;
+        }
+    }
+  };
+  if (AHEAD) fetch(row);
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * rows; r0 < a.M; r0 += step, row += step, ++turn) {
+    float h[K][V], gv[K][V];
+    Raw<T, V> sv[JOIN ? K : 1];
+    bool kept[K][V];
+    if (!AHEAD) fetch(row);
+    next.z(a, c, row, key, thr, h, kept);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      gnext[k].open(gv[k]);
+      if (JOIN) sv[k] = snext[k];
+    }
+    const float m = mnext, rs = rnext;
+    if (AHEAD) fetch(row + step);
+    if (AHEAD && turn % FLUSH == FLUSH - 1) flush();
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        h[k][i] = (h[k][i] - m) * rs;
+        if constexpr (AHEAD) {
+          dw[k][i] = fmaf(gv[k][i], h[k][i], dw[k][i]);
+          db[k][i] += gv[k][i];
+        } else {
+          mine[(k * V + i) * threads] += gv[k][i] * h[k][i];
+          mine[((K + k) * V + i) * threads] += gv[k][i];
+        }
+        gv[k][i] *= w[k][i];
+      }
+    if (a.F % V == 0) {                     // (g is zero where a thread has no column)
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) { s1 += gv[k][i]; s2 = fmaf(gv[k][i], h[k][i], s2); }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? gv[k][i] : 0.f; s1 += e; s2 = fmaf(e, h[k][i], s2); }
+    }
+    if constexpr (TPR != 0) {
+      s1 = lanes_sum<TPR>(s1);
+      s2 = lanes_sum<TPR>(s2);
+    } else {
+      s1 = lanes_sum<64>(s1);
+      s2 = lanes_sum<64>(s2);
+      float(*slot)[2] = part[turn & 1] + first * (c.threads >> 6);
+      if (gs_lane() == 0) { slot[c.t >> 6][0] = s1; slot[c.t >> 6][1] = s2; }
+      __syncthreads();
+      const bool there = threadIdx.x % MAXW < c.threads >> 6;
+      s1 = lanes_sum<MAXW>(there ? slot[threadIdx.x % MAXW][0] : 0.f);
+      s2 = lanes_sum<MAXW>(there ? slot[threadIdx.x % MAXW][1] : 0.f);
+    }
+    s1 *= inv_f;
+    s2 *= inv_f;
+    if constexpr (NT) settle();
+    if (row < a.M) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!c.on[k]) continue;
+        float o[V], q[V];
+        if (JOIN) sv[k].open(q);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          o[i] = rs * fmaf(-h[k][i], s2, gv[k][i] - s1);
+          if (JOIN) o[i] += q[i];
+        }
+        if (JOIN && d.gres) Raw<T, V>::template store<NT>(d.gres + row * a.F + c.col[k], o);
+        if (d.gx) {
+          if (JOIN && a.d.p > 0.f) drop_vec<V>(o, kept[k], a.d.inv_keep);
+          Raw<T, V>::template store<NT>(d.gx + row * a.F + c.col[k], o);
+        }
+      }
+    }
+    if constexpr (NT) settle();
+  }
+  if (!d.ws) return;
+  flush();
+  __syncthreads();
+  // this workgroup's column sums -> its slab, or (one workgroup) the result: element e of thread t's columns, over the
+  // threads of the workgroup's rows that hold the same columns
+  float *slab = d.ws + (int64_t)blockIdx.x * 2 * a.F;
+  for (int j = threadIdx.x; j < K * V * c.threads; j += blockDim.x) {
+    const int t = j % c.threads, e = j / c.threads, v = (t + e / V * c.threads) * V, at = v < a.F - V ? v : a.F - V;
+    if (v >= a.F || e % V < v - at) continue;
+    float u = 0.f, q = 0.f;
+    for (int r = 0; r < rows; ++r) {
+      u += acc[e * threads + r * c.threads + t];
+      q += acc[(K * V + e) * threads + r * c.threads + t];
+    }
+    const int col = at + e % V;
+    if (gridDim.x > 1) { slab[col] = u; slab[a.F + col] = q; continue; }
+    if (d.gw) store_w(d.gw, a.wdtype, col, u);
+    if (d.gb) store_w(d.gb, a.wdtype, col, q);
+  }
+}
+
+// The slabs' sum, in slab order per thread and in double: 16 columns of the 2 F a workgroup, 64 slabs at a time
+__global__ void __launch_bounds__(1024) ln_slabs_k(const float *ws, int slabs, int F, int wdtype, void *gw, void *gb) {
+  __shared__ double part[64][16];
+  const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+  const int s0 = threadIdx.x >> 4;
+  double v = 0.;
+  if (c < 2 * (int64_t)F)
+#pragma unroll 8
+    for (int s = s0; s < slabs; s += 64) v += (double)ws[(int64_t)s * 2 * F + c];
+  part[s0][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (threadIdx.x < 16 && c < 2 * (int64_t)F) {
+    v = 0.;
+    for (int s = 0; s < 64; ++s) v += part[s][threadIdx.x];
+    if (c < F) { if (gw) store_w(gw, wdtype, c, (float)v); }
+    else if (gb) store_w(gb, wdtype, c - F, (float)v);
+  }
+}
+
+// ------------------------------------------------------------------ rows longer than a workgroup's registers
+__device__ __forceinline__ float block_sum(float v) {      // over 1024 threads, in every thread
+  __shared__ float part[16];
+  v = lanes_sum<64>(v);
+  __syncthreads();
+  if (gs_lane() == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v += part[i];
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ float long_z(const Ln<T> &a, int64_t idx, uint64_t key) {
+  float v = (float)a.x[idx];
+  if (a.d.p > 0.f) v = dropout_keep(key, (uint64_t)idx, a.d.p) ? v * a.d.inv_keep : 0.f;
+  return a.res ? (float)a.res[idx] + v : v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) ln_fwd_long_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
+  const uint64_t key = drop_key(a.d);
+  const float inv_f = 1.0f / (float)a.F;
+  for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
+    const int64_t base = r * a.F;
+    float s = 0.f, q = 0.f;
+    for (int c = threadIdx.x; c < a.F; c += 1024) s += long_z(a, base + c, key);
+    const float m = block_sum(s) * inv_f;
+    for (int c = threadIdx.x; c < a.F; c += 1024) { const float e = long_z(a, base + c, key) - m; q = fmaf(e, e, q); }
+    const float rs = 1.0f / sqrtf(block_sum(q) * inv_f + eps);
+    for (int c = threadIdx.x; c < a.F; c += 1024) {
+      const float z = long_z(a, base + c, key);
+      float w[1] = {1.f}, b[1] = {0.f};
+      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
+      if (a.b) load_w<T, 1>(a.b, a.wdtype, c, b);
+      y[base + c] = (T)fmaf((z - m) * rs, w[0], b[0]);
+      if (sum) sum[base + c] = (T)z;
+    }
+    if (mean && threadIdx.x == 0) { mean[r] = m; rstd[r] = rs; }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const T *gsum, const float *mean,
+                                                     const float *rstd, T *gx, T *gres) {
+  const uint64_t key = drop_key(a.d);
+  const float inv_f = 1.0f / (float)a.F;
+  for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
+    const int64_t base = r * a.F;
+    const float m = mean[r], rs = rstd[r];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < a.F; c += 1024) {
+      const float h = (long_z(a, base + c, key) - m) * rs;
+      float w[1] = {1.f};
+      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
+      const float e = (float)g[base + c] * w[0];
+      s1 += e;
+      s2 = fmaf(e, h, s2);
+    }
+    s1 = block_sum(s1) * inv_f;
+    s2 = block_sum(s2) * inv_f;
+    for (int c = threadIdx.x; c < a.F; c += 1024) {
+      const int64_t i = base + c;
+      const float h = (long_z(a, i, key) - m) * rs;
+      float w[1] = {1.f};
+      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
+      const float e = (float)g[i] * w[0];
+      float dz = rs * (e - s1 - h * s2);
+      if (gsum) dz += (float)gsum[i];
+      if (gres) gres[i] = (T)dz;
+      if (gx) gx[i] = (T)(a.d.p <= 0.f ? dz : dropout_keep(key, (uint64_t)i, a.d.p) ? dz * a.d.inv_keep : 0.f);
+    }
+  }
+}
+
+// acc + v with the error carried on
+__device__ __forceinline__ void add_carry(float &acc, float &carry, float v) {
+  const float y = v - carry, t = acc + y;
+  carry = (t - acc) - y;
+  acc = t;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const float *mean, const float *rstd, float *ws) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.F) return;
+  const uint64_t key = drop_key(a.d);
+  float dw = 0.f, db = 0.f, dwc = 0.f, dbc = 0.f;
+  for (int64_t r = blockIdx.y; r < a.M; r += gridDim.y) {
+    const float gv = (float)g[r * a.F + c];
+    add_carry(dw, dwc, gv * ((long_z(a, r * a.F + c, key) - mean[r]) * rstd[r]));
+    add_carry(db, dbc, gv);
+  }
+  float *slab = ws + (int64_t)blockIdx.y * 2 * a.F;
+  slab[c] = dw;
+  slab[a.F + c] = db;
+}
+
+// ------------------------------------------------------------------ launches
+// Workgroups of this kernel that the GPU holds at once: the rows are dealt out to these, none waits for a place
+template <auto KERNEL> int ln_resident(int threads, int lds) {
+  static std::atomic<int> known[MAXW + 1];
+  std::atomic<int> &n = known[threads / 64];
+  int blocks = n.load(std::memory_order_relaxed);
+  if (blocks == 0) {
+    if (lds > 65536) (void)hipFuncSetAttribute((const void *)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, KERNEL, threads, lds) != hipSuccess || blocks < 1) blocks = 1;
+    n.store(blocks, std::memory_order_relaxed);
+  }
+  return 256 * blocks;
+}
+
+// Tables too large for any cache (256 MB behind the L2s) are read and written past them: 10 M x 64 fp32 forward
+// 1.09 -> 1.03 ms, backward 1.55 -> 1.51, joined 1.86 -> 1.68 and 3.00 -> 2.89 ms; a 15 MB table loses that way (7.1 ->
+// 11.8 us), for the caches serve it, and so do rows that share cache lines (400 M x 196 fp16 joined forward 4.7 -> 4.1 TB/s).
+bool streams(int64_t n, size_t size) { return n * (int64_t)size >= ((int64_t)256 << 20); }
+bool whole_lines(int64_t F, size_t size) { return F * (int64_t)size % 128 == 0; }
+
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
+  constexpr auto kernel = ln_fwd_k<T, V, TPR, K, JOIN, NT>;
+  const int threads = TPR ? 256 : a.row;
+  hipLaunchKernelGGL(kernel, dim3(norm_blocks(a.M, threads / a.row, ln_resident<kernel>(threads, 0))), dim3(threads), 0, st,
+                     a, eps, y, sum, mean, rstd);
+}
+
+// -> the workgroups launched: as many slabs of column sums
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
+  constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT>;
+  const int rows = ln_bwd_threads(V, TPR, K) / a.row, threads = rows * a.row;
+  constexpr int lds = 2 * K * V * ln_bwd_threads(V, TPR, K) * (int)sizeof(float);
+  const int resident = ln_resident<kernel>(threads, lds), most = norm_max_slabs(a.M, a.F);
+  // (of the large tables sixteen waves a compute unit keep the memory busy; 24 of them were slower: 1.49 against 1.41 ms)
+  const int held = NT && resident > 512 ? 512 : resident;
+  const int slabs = norm_blocks(a.M, rows, held < most ? held : most);
+  hipLaunchKernelGGL(kernel, dim3(slabs), dim3(threads), lds, st, a, d);
+  return slabs;
+}
+
+// every form: CASE(kind, V, TPR, K); LINE: those of large plain tables only
+#define LN_FORMS(CASE, LINE)                                                                                  \
+  CASE(NORM_ONE, 1, 8, 1) CASE(NORM_R4, V, 4, 1) CASE(NORM_R8, V, 8, 1) CASE(NORM_R8x2, V, 8, 2)              \
+  CASE(NORM_R8x3, V, 8, 3) LINE(NORM_R16, V, 16, 1) CASE(NORM_R16x2, V, 16, 2) CASE(NORM_R16x3, V, 16, 3)     \
+  LINE(NORM_R32, V, 32, 1) CASE(NORM_R32x2, V, 32, 2) CASE(NORM_R32x3, V, 32, 3) LINE(NORM_R64, V, 64, 1)     \
+  CASE(NORM_R64x2, V, 64, 2) CASE(NORM_R64x3, V, 64, 3) CASE(NORM_B2, V, 0, 2) CASE(NORM_B3, V, 0, 3) CASE(NORM_B4, V, 0, 4)
+
+template <typename T>
+int ln_fwd(const NormFwd &n, hipStream_t st) {
+  constexpr int V = Tab<T>::V;
+  const bool join = n.res || n.d.p > 0.f || n.sum, nt = streams(n.M * n.F, sizeof(T)) && whole_lines(n.F, sizeof(T));
+  const NormForm f = norm_form(n.F, V, nt && !join);
+  const Ln<T> a{(const T *)n.x, (const T *)n.res, n.w, n.b, n.M, (int)n.F, n.wdtype, f.row, n.d};
+  T *y = (T *)n.y, *sum = (T *)n.sum;
+#define ARGS a, n.eps, y, sum, n.mean, n.rstd, st
+#define CASE(KIND, V, TPR, K)                                                                        \
+  case KIND:                                                                                         \
+    if (join) { if (nt) ln_fwd_go<T, V, TPR, K, true, true>(ARGS); else ln_fwd_go<T, V, TPR, K, true, false>(ARGS); } \
+    else { if (nt) ln_fwd_go<T, V, TPR, K, false, true>(ARGS); else ln_fwd_go<T, V, TPR, K, false, false>(ARGS); }    \
+    break;
+#define LINE(KIND, V, TPR, K) \
+  case KIND: ln_fwd_go<T, V, TPR, K, false, true>(ARGS); break;
+  switch (f.kind) {
+    LN_FORMS(CASE, LINE)
+    case NORM_B8:
+      if constexpr (V == 4) {
+        if (join) ln_fwd_go<T, V, 0, 8, true, false>(ARGS);
+        else ln_fwd_go<T, V, 0, 8, false, false>(ARGS);
+      }
+      break;
+    case NORM_LONG:
+      hipLaunchKernelGGL(ln_fwd_long_k<T>, dim3(gs_grid(n.M, 1, 512)), dim3(1024), 0, st, a, n.eps, y, sum, n.mean, n.rstd);
+  }
+#undef CASE
+#undef LINE
+#undef ARGS
+  GSAGE_CHECK_LAUNCH();
+  return GSAGE_OK;
+}
+
+template <typename T>
+int ln_bwd(const NormBwd &n, hipStream_t st) {
+  constexpr int V = Tab<T>::V;
+  const bool join = n.res || n.d.p > 0.f || n.gsum || n.gres, nt = streams(n.M * n.F, sizeof(T)) && whole_lines(n.F, sizeof(T));
+  const NormForm f = norm_form(n.F, V, nt && !join);
+  const Ln<T> a{(const T *)n.x, (const T *)n.res, n.w, nullptr, n.M, (int)n.F, n.wdtype, f.row, n.d};
+  const Grads<T> d{(const T *)n.g, (const T *)n.gsum, n.mean, n.rstd, (T *)n.gx, (T *)n.gres,
+                   n.gw || n.gb ? n.ws : nullptr, n.gw, n.gb};
+  int slabs = norm_max_slabs(n.M, n.F);
+  if (n.M > 0 && (d.gx || d.gres || d.ws)) {
+#define CASE(KIND, V, TPR, K)                                                                          \
+  case KIND:                                                                                           \
+    slabs = join ? (nt ? ln_bwd_go<T, V, TPR, K, true, true>(a, d, st) : ln_bwd_go<T, V, TPR, K, true, false>(a, d, st))   \
+                 : (nt ? ln_bwd_go<T, V, TPR, K, false, true>(a, d, st) : ln_bwd_go<T, V, TPR, K, false, false>(a, d, st)); \
+    break;
+#define LINE(KIND, V, TPR, K) \
+  case KIND: slabs = ln_bwd_go<T, V, TPR, K, false, true>(a, d, st); break;
+    switch (f.kind) {
+      LN_FORMS(CASE, LINE)
+      case NORM_B8:
+        if constexpr (V == 4)
+          slabs = join ? ln_bwd_go<T, V, 0, 8, true, false>(a, d, st) : ln_bwd_go<T, V, 0, 8, false, false>(a, d, st);
+        break;
+      case NORM_LONG:
+        if (d.gx || d.gres)
+          hipLaunchKernelGGL(ln_dz_long_k<T>, dim3(gs_grid(n.M, 1, 512)), dim3(1024), 0, st, a, d.g, d.gsum, d.mean, d.rstd,
+                             d.gx, d.gres);
+        if (d.ws)
+          hipLaunchKernelGGL(ln_dw_long_k<T>, dim3((unsigned)((n.F + 255) / 256), slabs), dim3(256), 0, st, a, d.g, d.mean,
+                             d.rstd, d.ws);
+    }
+#undef CASE
+#undef LINE
+    GSAGE_CHECK_LAUNCH();
+  }
+  if (d.ws && (slabs != 1 || f.kind == NORM_LONG)) {
+    hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * n.F + 15) / 16)), dim3(1024), 0, st, d.ws, slabs, (int)n.F, n.wdtype,
+                       d.gw, d.gb);
+    GSAGE_CHECK_LAUNCH();
+  }
+  return GSAGE_OK;
+}
+
+template <typename T> int dropout_go(const void *x, int64_t n, const NormDrop &d, void *out, hipStream_t st) {
+  const dim3 grid(gs_grid(n, 256 * 16)), block(256);
+  if (streams(n, sizeof(T))) hipLaunchKernelGGL((dropout_k<T, true>), grid, block, 0, st, (const T *)x, n, d, (T *)out);
+  else hipLaunchKernelGGL((dropout_k<T, false>), grid, block, 0, st, (const T *)x, n, d, (T *)out);
+  GSAGE_CHECK_LAUNCH();
+  return GSAGE_OK;
+}
+
+}  // namespace
