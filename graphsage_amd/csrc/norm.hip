@@ -38,9 +38,8 @@ extern "C" int gsage_layer_norm_fwd(const void *x, const void *residual, const v
 }
 
 extern "C" size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype) {
-  if (M < 0 || F <= 0 || F > MAX_F || bad_dtype(dtype)) return 0;
-  const size_t slabs = (size_t)norm_max_slabs(M, F);
-  return gs_align_up((slabs ? slabs : 1) * 2 * (size_t)F * sizeof(float), 256);
+  if (M < 0 || F <= 0 || F > MAX_F || M > MAX_N / F || bad_dtype(dtype)) return 0;
+  return gs_align_up((size_t)norm_ws_floats(M, F, dtype == GSAGE_F32 ? 4 : 2) * sizeof(float), 256);
 }
 
 extern "C" int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, const void *x, const void *residual,

@@ -83,7 +83,10 @@ template <> struct Tab<_Float16> {
 // NT: accesses that are not to be kept in the caches
 template <typename T, int V> struct Raw {
   u32x4 w;
-  __device__ __forceinline__ void zero() { w = u32x4{0u, 0u, 0u, 0u}; }
+  __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = on ? w[i] : 0u;
+  }
   template <bool NT = false> __device__ __forceinline__ void load(const T *p) {
     const auto *q = (const typename Tab<T>::mem *)p;
     if constexpr (NT) w = __builtin_nontemporal_load(q);
@@ -98,7 +101,7 @@ template <typename T, int V> struct Raw {
 };
 template <typename T> struct Raw<T, 1> {
   T w;
-  __device__ __forceinline__ void zero() { w = (T)0.f; }
+  __device__ __forceinline__ void keep(bool on) { w = on ? w : (T)0.f; }
   template <bool NT = false> __device__ __forceinline__ void load(const T *p) { w = *p; }
   __device__ __forceinline__ void open(float (&f)[1]) const { f[0] = (float)w; }
   template <bool NT = false> static __device__ __forceinline__ void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
@@ -125,35 +128,27 @@ template <int V> __device__ __forceinline__ void drop_vec(float (&f)[V], const b
   for (int i = 0; i < V; ++i) f[i] = kept[i] ? f[i] * inv_keep : 0.f;
 }
 
+// A vector a thread and as many workgroups as that takes: they start in order, so at any time the GPU reads and writes one
+// short stretch of each table, and the memory stays on its open pages.  The same loop over a grid the GPU holds at once,
+// whose workgroups drift apart, reaches three quarters of it (10 M x 64 fp32: 0.80 ms, 6.4 TB/s; 1.11 ms with four vectors
+// a turn, 1.00 with one).
 template <typename T, bool NT>
-__global__ void __launch_bounds__(256) dropout_k(const T *x, int64_t n, NormDrop d, T *out) {
-  constexpr int V = Tab<T>::V, U = 4;
+__global__ void __launch_bounds__(256) dropout_k(const T *x, int64_t n, int64_t begin, NormDrop d, T *out) {
+  constexpr int V = Tab<T>::V;
   const uint64_t key = drop_key(d);
   const uint32_t thr = dropout_threshold(d.p);
-  const int64_t nv = n / V, stride = (int64_t)gridDim.x * 256;
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const auto put = [&](const Raw<T, V> &r, int64_t at) {
-    float f[V];
-    bool kept[V];
-    r.open(f);
-    draw_vec<V>(kept, (uint64_t)at * V, key, thr, d.p);
-    drop_vec<V>(f, kept, d.inv_keep);
-    Raw<T, V>::template store<NT>(out + at * V, f);
-  };
-  for (; i + (U - 1) * stride < nv; i += U * stride) {
-    Raw<T, V> r[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) r[u].template load<NT>(x + (i + u * stride) * V);
-#pragma unroll
-    for (int u = 0; u < U; ++u) put(r[u], i + u * stride);
-  }
-  for (; i < nv; i += stride) {
+  const int64_t i = begin + (int64_t)blockIdx.x * 256 + threadIdx.x, nv = n / V;
+  if (i < nv) {
     Raw<T, V> r;
     r.template load<NT>(x + i * V);
-    put(r, i);
-  }
-  if (blockIdx.x == 0 && threadIdx.x < n - nv * V) {      // the last n mod V elements
-    const int64_t e = nv * V + threadIdx.x;
+    float f[V];
+    bool kept[V];
+    draw_vec<V>(kept, (uint64_t)i * V, key, thr, d.p);
+    r.open(f);
+    drop_vec<V>(f, kept, d.inv_keep);
+    Raw<T, V>::template store<NT>(out + i * V, f);
+  } else if (i - nv < n - nv * V) {      // the last n mod V elements
+    const int64_t e = nv * V + (i - nv);
     out[e] = (T)(dropout_keep(key, (uint64_t)e, d.p) ? (float)x[e] * d.inv_keep : 0.f);
   }
 }
@@ -179,28 +174,32 @@ template <int N> __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// V weights from column c on, fp32 or of the tables' type
-template <typename T, int V> __device__ __forceinline__ void load_w(const void *w, int wdtype, int c, float (&f)[V]) {
-  if (wdtype == GSAGE_F32) {
-    const float *p = (const float *)w + c;
-    if constexpr (V == 1) f[0] = p[0];
-    else {
-#pragma unroll
-      for (int q = 0; q < V; q += 4) {
-        float o[4];
-        Raw<float, 4> r;
-        r.load(p + q);
-        r.open(o);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[q + i] = o[i];
-      }
-    }
-  } else {
-    Raw<T, V> r;
-    r.load((const T *)w + c);
-    r.open(f);
+// V weights from a column on, fp32 or of the tables' type: loaded in one place, made fp32 in another, so that the loads
+// of a row's operands go out between (NULL: `other` V times)
+template <typename T, int V> struct Weights {
+  u32x4 r[V > 4 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *w, int wdtype, int c) {
+    if (!w) return;
+    if constexpr (V == 1) {
+      if (wdtype == GSAGE_F32) r[0][0] = as_u(((const float *)w)[c]);
+      else r[0][0] = as_u((float)((const T *)w)[c]);
+    } else if (wdtype == GSAGE_F32) {
+      const float *p = (const float *)w + c;
+      r[0] = *(const Tab<float>::mem *)p;
+      if constexpr (V > 4) r[1] = *(const Tab<float>::mem *)(p + 4);
+    } else r[0] = *(const typename Tab<T>::mem *)((const T *)w + c);
   }
-}
+  __device__ __forceinline__ void open(const void *w, int wdtype, float other, float (&f)[V]) const {
+    if (!w) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = other;
+    } else if constexpr (V == 1) f[0] = as_f(r[0][0]);
+    else if (wdtype == GSAGE_F32) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = as_f(r[i / 4][i % 4]);
+    } else Tab<T>::open(r[0], f);
+  }
+};
 __device__ __forceinline__ void store_w(void *w, int wdtype, int64_t c, float v) {
   if (wdtype == GSAGE_F32) ((float *)w)[c] = v;
   else if (wdtype == GSAGE_BF16) ((__bf16 *)w)[c] = (__bf16)v;
@@ -249,78 +248,88 @@ template <int V, int TPR, int K> struct Cols {
   }
 };
 
-// The operands of z of one row: loaded a row ahead of their use (short rows), or at it
+// The operands of z of one row.  Loaded without a branch a vector: where a thread has no column it loads its neighbour's
+// (and row `row` must be one of the table's), and drops it at use.
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT> struct Operands {
   Raw<T, V> x[K], r[JOIN ? K : 1];
-  __device__ __forceinline__ void load(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, bool in) {
+  __device__ __forceinline__ void load(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      x[k].zero();
-      if (JOIN) r[k].zero();
-      if (in && c.on[k]) {
-        x[k].template load<NT>(a.x + row * a.F + c.col[k]);
-        if (JOIN && a.res) r[k].template load<NT>(a.res + row * a.F + c.col[k]);
-      }
-    }
+    for (int k = 0; k < K; ++k) x[k].template load<NT>(a.x + row * a.F + c.col[k]);
+    if (JOIN && a.res)
+#pragma unroll
+      for (int k = 0; k < K; ++k) r[k].template load<NT>(a.res + row * a.F + c.col[k]);
   }
+  // (zero where the thread has no column)
   __device__ __forceinline__ void z(const Ln<T> &a, const Cols<V, TPR, K> &c, int64_t row, uint64_t key, uint32_t thr,
-                                    float (&z)[K][V], bool (&kept)[K][V]) const {
+                                    float (&z)[K][V], bool (&kept)[K][V]) {
+    if (!c.full)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        x[k].keep(c.on[k]);
+        if (JOIN) r[k].keep(c.on[k]);
+      }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       x[k].open(z[k]);
-      if (JOIN) {
-        if (a.d.p > 0.f) {
-          draw_vec<V>(kept[k], (uint64_t)(row * a.F + c.col[k]), key, thr, a.d.p);
-          drop_vec<V>(z[k], kept[k], a.d.inv_keep);
-        }
-        if (a.res) {
-          float q[V];
-          r[k].open(q);
-#pragma unroll
-          for (int i = 0; i < V; ++i) z[k][i] += q[i];
-        }
+      if (JOIN && a.d.p > 0.f) {
+        draw_vec<V>(kept[k], (uint64_t)(row * a.F + c.col[k]), key, thr, a.d.p);
+        drop_vec<V>(z[k], kept[k], a.d.inv_keep);
       }
     }
+    if (JOIN && a.res)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float q[V];
+        r[k].open(q);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[k][i] += q[i];
+      }
   }
 };
 
-// Nothing of this wave is under way (vmcnt = 0).  Streaming kernels wait so before their stores and after them: reads and
-// writes then come in turns, which the memory takes better than both at once (10 M x 64 fp32 forward 0.94 against
-// 0.99 ms; joined backward 2.36 against 2.50 ms, 1 M x 256 0.87 against 0.97).
-__device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// Rows of a workgroup: those it takes at once from begin + blockIdx apart on, then `step` further for each of `turns`
+struct Walk { int64_t begin, apart, step; int turns; };
 
 // ------------------------------------------------------------------ forward
-template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
-__global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW, NT && K == 1 ? 8 : 1) ln_fwd_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
-  constexpr bool AHEAD = K * V < 32;          // 32 elements a thread: no registers left for the row after
+// LOOP: several turns, the row after in flight; otherwise one turn and as many workgroups as that takes, which start in
+// order (see dropout_k: 1 M x 128 fp32 0.165 ms, 0.178 as a loop over the grid the GPU holds, joined 0.237 and 0.272).
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT, bool LOOP>
+__global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW) ln_fwd_k(Ln<T> a, Walk g, float eps, T *y, T *sum, float *mean, float *rstd) {
+  constexpr bool AHEAD = LOOP && K * V < 32;  // 32 elements a thread: no registers left for the row after
   __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
   const Cols<V, TPR, K> c(a.F, a.row);
-  const int rows = TPR ? 256 / (TPR ? TPR : 1) : 1, first = TPR ? threadIdx.x / (TPR ? TPR : 1) : 0;   // rows at once, this thread's
+  const int first = TPR ? threadIdx.x / (TPR ? TPR : 1) : 0;      // this thread's among the rows at once
+  int64_t row = g.begin + (int64_t)blockIdx.x * g.apart + first;
+  Operands<T, V, TPR, K, JOIN, NT> next;
+  const auto fetch = [&](int64_t r) { next.load(a, c, r < a.M ? r : a.M - 1); };
+  fetch(row);
+  Weights<T, V> wr[K], br[K];
   float w[K][V], b[K][V];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
+  for (int k = 0; k < K; ++k) wr[k].load(a.w, a.wdtype, c.col[k]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) { w[k][i] = 1.f; b[k][i] = 0.f; }
-    if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
-    if (a.b && c.on[k]) load_w<T, V>(a.b, a.wdtype, c.col[k], b[k]);
-  }
+  for (int k = 0; k < K; ++k) br[k].load(a.b, a.wdtype, c.col[k]);
+  const auto weights = [&]() {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      wr[k].open(a.w, a.wdtype, 1.f, w[k]);
+      br[k].open(a.b, a.wdtype, 0.f, b[k]);
+    }
+  };
   const uint64_t key = JOIN ? drop_key(a.d) : 0;
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
   // (rows of several waves) this wave's elements, and those of the wave whose sums this lane puts together
   const int mine = TPR ? 0 : c.wave_count(c.t >> 6, a.F), other = TPR ? 0 : c.wave_count(threadIdx.x % MAXW, a.F);
   const float inv_mine = mine ? 1.0f / (float)mine : 0.f, inv_other = other ? 1.0f / (float)other : 0.f;
-  const int64_t step = (int64_t)gridDim.x * rows;
-  int64_t row = (int64_t)blockIdx.x * rows + first;
-  Operands<T, V, TPR, K, JOIN, NT> next;
-  if (AHEAD) next.load(a, c, row, row < a.M);
-  int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * rows; r0 < a.M; r0 += step, row += step, turn ^= 1) {
+  if (LOOP) weights();
+  const int turns = LOOP ? g.turns : 1;
+  for (int turn = 0; turn < turns; ++turn, row += g.step) {
     float z[K][V];
     bool kept[K][V];
-    if (!AHEAD) next.load(a, c, row, row < a.M);
+    if (!AHEAD && turn > 0) fetch(row);
     next.z(a, c, row, key, thr, z, kept);
-    if (AHEAD) next.load(a, c, row + step, row + step < a.M);
+    if (AHEAD && turn + 1 < turns) fetch(row + g.step);
     float s = 0.f, q = 0.f, m, var;
     const auto squares = [&](float about) {
       if (c.full) {
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW, NT && K == 1 
       const float sw = lanes_sum<64>(s);
       squares(sw * inv_mine);
       q = lanes_sum<64>(q);
-      float(*slot)[2] = part[turn];
+      float(*slot)[2] = part[turn & 1];
       if (gs_lane() == 0) { slot[c.t >> 6][0] = sw; slot[c.t >> 6][1] = q; }
       __syncthreads();
       // (waves that are not there have no elements; their slots hold whatever LDS held)
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW, NT && K == 1 
       var = lanes_sum<MAXW>(fmaf(e * e, (float)other, qo)) * inv_f;
     }
     const float rs = rsqrtf(var + eps);
-    if constexpr (NT) settle();
+    if (!LOOP) weights();
     if (row < a.M) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -380,7 +389,6 @@ __global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW, NT && K == 1 
       }
       if (mean && c.t == 0) { mean[row] = m; rstd[row] = rs; }
     }
-    if constexpr (NT) settle();
   }
 }
 
@@ -406,8 +414,13 @@ constexpr bool ln_bwd_ahead(int V, int TPR, int K, bool JOIN) {
 }
 constexpr int ln_bwd_threads(int V, int TPR, int K) { return K == 3 && V == 8 && TPR == 0 ? 256 : 64 * MAXW; }
 
+// Nothing of this wave is under way (vmcnt = 0).  The loops over the grid that the GPU holds wait so before their stores and
+// after them on streamed tables: reads and writes then come in turns, which the memory takes better than both at once
+// (10 M x 64 fp32 joined backward 2.36 against 2.50 ms, 1 M x 256 0.87 against 0.97).
+__device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
-__global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, Grads<T> d) {
+__global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, Walk g, Grads<T> d) {
   constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
   constexpr int A = AHEAD ? K : 1;
   extern __shared__ float acc[];              // [2 K V][threads]: grad_w, then grad_b; a thread's words are its own
@@ -416,40 +429,38 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, G
   float *const mine = acc + threadIdx.x;
   const Cols<V, TPR, K> c(a.F, a.row);
   const int rows = TPR ? threads / (TPR ? TPR : 1) : blockDim.x / c.threads, first = threadIdx.x / c.threads;
+  int64_t base = g.begin + (int64_t)blockIdx.x * g.apart, row = base + first;
+  Operands<T, V, TPR, K, JOIN, NT> next;
+  Raw<T, V> gnext[K], snext[JOIN ? K : 1];
+  float mnext, rnext;
+  const auto fetch = [&](int64_t at) {
+    const int64_t r = at < a.M ? at : a.M - 1;
+    next.load(a, c, r);
+#pragma unroll
+    for (int k = 0; k < K; ++k) gnext[k].template load<NT>(d.g + r * a.F + c.col[k]);
+    if (JOIN && d.gsum)
+#pragma unroll
+      for (int k = 0; k < K; ++k) snext[k].template load<NT>(d.gsum + r * a.F + c.col[k]);
+    mnext = d.mean[r];
+    rnext = d.rstd[r];
+  };
+  fetch(row);
+  Weights<T, V> wr[K];
   float w[K][V], dw[A][V], db[A][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) wr[k].load(a.w, a.wdtype, c.col[k]);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      w[k][i] = 1.f;
       if (AHEAD) dw[k % A][i] = db[k % A][i] = 0.f;
       mine[(k * V + i) * threads] = mine[((K + k) * V + i) * threads] = 0.f;
     }
-    if (a.w && c.on[k]) load_w<T, V>(a.w, a.wdtype, c.col[k], w[k]);
+    wr[k].open(a.w, a.wdtype, 1.f, w[k]);
   }
   const uint64_t key = JOIN ? drop_key(a.d) : 0;
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
-  const int64_t step = (int64_t)gridDim.x * rows;
-  int64_t row = (int64_t)blockIdx.x * rows + first;
-  Operands<T, V, TPR, K, JOIN, NT> next;
-  Raw<T, V> gnext[K], snext[JOIN ? K : 1];
-  float mnext = 0.f, rnext = 0.f;
-  const auto fetch = [&](int64_t r) {
-    const bool in = r < a.M;
-    next.load(a, c, r, in);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      gnext[k].zero();
-      if (JOIN) snext[k].zero();
-      if (in && c.on[k]) {
-        gnext[k].template load<NT>(d.g + r * a.F + c.col[k]);
-        if (JOIN && d.gsum) snext[k].template load<NT>(d.gsum + r * a.F + c.col[k]);
-      }
-    }
-    mnext = in ? d.mean[r] : 0.f;
-    rnext = in ? d.rstd[r] : 0.f;
-  };
   const auto flush = [&]() {
     if constexpr (AHEAD) {
 #pragma unroll
@@ -462,21 +473,22 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, G
         }
     }
   };
-  if (AHEAD) fetch(row);
-  int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * rows; r0 < a.M; r0 += step, row += step, ++turn) {
+  for (int turn = 0; turn < g.turns; ++turn, base += g.step, row += g.step) {
     float h[K][V], gv[K][V];
     Raw<T, V> sv[JOIN ? K : 1];
     bool kept[K][V];
-    if (!AHEAD) fetch(row);
+    if (!AHEAD && turn > 0) fetch(row);
     next.z(a, c, row, key, thr, h, kept);
+    if (!c.full || base + rows > a.M)                             // no column, or no row: nothing for the sums
+#pragma unroll
+      for (int k = 0; k < K; ++k) gnext[k].keep(c.on[k] && row < a.M);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       gnext[k].open(gv[k]);
       if (JOIN) sv[k] = snext[k];
     }
     const float m = mnext, rs = rnext;
-    if (AHEAD) fetch(row + step);
+    if (AHEAD && turn + 1 < g.turns) fetch(row + g.step);
     if (AHEAD && turn % FLUSH == FLUSH - 1) flush();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -524,12 +536,14 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, G
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!c.on[k]) continue;
-        float o[V], q[V];
-        if (JOIN) sv[k].open(q);
+        float o[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          o[i] = rs * fmaf(-h[k][i], s2, gv[k][i] - s1);
-          if (JOIN) o[i] += q[i];
+        for (int i = 0; i < V; ++i) o[i] = rs * fmaf(-h[k][i], s2, gv[k][i] - s1);
+        if (JOIN && d.gsum) {
+          float q[V];
+          sv[k].open(q);
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] += q[i];
         }
         if (JOIN && d.gres) Raw<T, V>::template store<NT>(d.gres + row * a.F + c.col[k], o);
         if (d.gx) {
@@ -558,6 +572,24 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, G
     if (gridDim.x > 1) { slab[col] = u; slab[a.F + col] = q; continue; }
     if (d.gw) store_w(d.gw, a.wdtype, col, u);
     if (d.gb) store_w(d.gb, a.wdtype, col, q);
+  }
+}
+
+// Thousands of slabs -> gridDim.y of them: 64 columns of the 2 F a workgroup, `per` slabs
+__global__ void __launch_bounds__(1024) ln_fold_k(const float *ws, int slabs, int per, int F, float *out) {
+  __shared__ double part[16][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + gs_lane();
+  const int s0 = blockIdx.y * per, s1 = s0 + per < slabs ? s0 + per : slabs, w = threadIdx.x >> 6;
+  double v = 0.;
+  if (c < 2 * (int64_t)F)
+#pragma unroll 8
+    for (int s = s0 + w; s < s1; s += 16) v += (double)ws[(int64_t)s * 2 * F + c];
+  part[w][gs_lane()] = v;
+  __syncthreads();
+  if (w == 0 && c < 2 * (int64_t)F) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += part[i][gs_lane()];
+    out[(int64_t)blockIdx.y * 2 * F + c] = (float)v;
   }
 }
 
@@ -593,6 +625,14 @@ __device__ __forceinline__ float block_sum(float v) {      // over 1024 threads,
   return v;
 }
 
+template <typename T> __device__ __forceinline__ float weight1(const void *w, int wdtype, int c, float other) {
+  Weights<T, 1> r;
+  float f[1];
+  r.load(w, wdtype, c);
+  r.open(w, wdtype, other, f);
+  return f[0];
+}
+
 template <typename T> __device__ __forceinline__ float long_z(const Ln<T> &a, int64_t idx, uint64_t key) {
   float v = (float)a.x[idx];
   if (a.d.p > 0.f) v = dropout_keep(key, (uint64_t)idx, a.d.p) ? v * a.d.inv_keep : 0.f;
@@ -612,10 +652,8 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_k(Ln<T> a, float eps, T *y, 
     const float rs = 1.0f / sqrtf(block_sum(q) * inv_f + eps);
     for (int c = threadIdx.x; c < a.F; c += 1024) {
       const float z = long_z(a, base + c, key);
-      float w[1] = {1.f}, b[1] = {0.f};
-      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
-      if (a.b) load_w<T, 1>(a.b, a.wdtype, c, b);
-      y[base + c] = (T)fmaf((z - m) * rs, w[0], b[0]);
+      const float w = weight1<T>(a.w, a.wdtype, c, 1.f), b = weight1<T>(a.b, a.wdtype, c, 0.f);
+      y[base + c] = (T)fmaf((z - m) * rs, w, b);
       if (sum) sum[base + c] = (T)z;
     }
     if (mean && threadIdx.x == 0) { mean[r] = m; rstd[r] = rs; }
@@ -633,9 +671,7 @@ __global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const 
     float s1 = 0.f, s2 = 0.f;
     for (int c = threadIdx.x; c < a.F; c += 1024) {
       const float h = (long_z(a, base + c, key) - m) * rs;
-      float w[1] = {1.f};
-      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
-      const float e = (float)g[base + c] * w[0];
+      const float e = (float)g[base + c] * weight1<T>(a.w, a.wdtype, c, 1.f);
       s1 += e;
       s2 = fmaf(e, h, s2);
     }
@@ -644,9 +680,7 @@ __global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const 
     for (int c = threadIdx.x; c < a.F; c += 1024) {
       const int64_t i = base + c;
       const float h = (long_z(a, i, key) - m) * rs;
-      float w[1] = {1.f};
-      if (a.w) load_w<T, 1>(a.w, a.wdtype, c, w);
-      const float e = (float)g[i] * w[0];
+      const float e = (float)g[i] * weight1<T>(a.w, a.wdtype, c, 1.f);
       float dz = rs * (e - s1 - h * s2);
       if (gsum) dz += (float)gsum[i];
       if (gres) gres[i] = (T)dz;
@@ -679,6 +713,8 @@ __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const f
 }
 
 // ------------------------------------------------------------------ launches
+constexpr int64_t MAX_GRID = 1 << 20;      // workgroups of a launch (a launch's threads are counted in 32 bits)
+
 // Workgroups of this kernel that the GPU holds at once: the rows are dealt out to these, none waits for a place
 template <auto KERNEL> int ln_resident(int threads, int lds) {
   static std::atomic<int> known[MAXW + 1];
@@ -692,32 +728,66 @@ template <auto KERNEL> int ln_resident(int threads, int lds) {
   return 256 * blocks;
 }
 
-// Tables too large for any cache (256 MB behind the L2s) are read and written past them: 10 M x 64 fp32 forward
-// 1.09 -> 1.03 ms, backward 1.55 -> 1.51, joined 1.86 -> 1.68 and 3.00 -> 2.89 ms; a 15 MB table loses that way (7.1 ->
-// 11.8 us), for the caches serve it, and so do rows that share cache lines (400 M x 196 fp16 joined forward 4.7 -> 4.1 TB/s).
-bool streams(int64_t n, size_t size) { return n * (int64_t)size >= ((int64_t)256 << 20); }
-bool whole_lines(int64_t F, size_t size) { return F * (int64_t)size % 128 == 0; }
-
-template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
-void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
-  constexpr auto kernel = ln_fwd_k<T, V, TPR, K, JOIN, NT>;
-  const int threads = TPR ? 256 : a.row;
-  hipLaunchKernelGGL(kernel, dim3(norm_blocks(a.M, threads / a.row, ln_resident<kernel>(threads, 0))), dim3(threads), 0, st,
-                     a, eps, y, sum, mean, rstd);
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT, bool LOOP>
+void ln_fwd_launch(const Ln<T> &a, int turns, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
+  constexpr auto kernel = ln_fwd_k<T, V, TPR, K, JOIN, NT, LOOP>;
+  const int threads = TPR ? 256 : a.row, rows = threads / a.row;
+  if (turns > 0) {      // neighbouring rows, workgroups in order
+    const int64_t apart = (int64_t)rows * turns;
+    for (int64_t begin = 0; begin < a.M; begin += MAX_GRID * apart) {
+      const int64_t left = (a.M - begin + apart - 1) / apart;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(left < MAX_GRID ? left : MAX_GRID)), dim3(threads), 0, st, a,
+                         Walk{begin, apart, rows, turns}, eps, y, sum, mean, rstd);
+    }
+  } else {              // the grid that the GPU holds
+    const int blocks = norm_blocks(a.M, rows, ln_resident<kernel>(threads, 0));
+    const int64_t step = (int64_t)blocks * rows;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, st, a, Walk{0, rows, step, (int)((a.M + step - 1) / step)}, eps, y,
+                       sum, mean, rstd);
+  }
 }
 
-// -> the workgroups launched: as many slabs of column sums
+// One turn a workgroup, where it has 3 KB of rows to spread its weights over; 16-bit rows without dropout or a residual
+// need two (less arithmetic a byte: 4 M x 64 bf16 0.165 against 0.191 ms), and so do rows of two or four waves.  Rows of
+// three waves and of 32 elements a thread run as loops over the grid that the GPU holds (8191 x 5120 bf16 33 us, 36 in
+// order; 8192 x 16000 100 us, 108).
+template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
+void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
+  const int64_t bytes = 256 / (TPR ? TPR : 256) * (int64_t)a.F * sizeof(T);
+  constexpr bool thin = sizeof(T) == 2 && !JOIN;
+  if constexpr (TPR == 0) ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, K == 2 ? 2 : 0, eps, y, sum, mean, rstd, st);
+  else if constexpr (thin || K == 1) {
+    if (thin || bytes < 3072)
+      ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, bytes < 4096 ? (int)((8191 + bytes) / bytes) : 2, eps, y, sum, mean, rstd, st);
+    else if constexpr (!thin) ln_fwd_launch<T, V, TPR, K, JOIN, NT, false>(a, 1, eps, y, sum, mean, rstd, st);
+  } else ln_fwd_launch<T, V, TPR, K, JOIN, NT, false>(a, 1, eps, y, sum, mean, rstd, st);
+}
+
+// -> the slabs of column sums that are left in ws
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
-  constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT>;
-  const int rows = ln_bwd_threads(V, TPR, K) / a.row, threads = rows * a.row;
+  constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT && K * V < 32>;      // (32 elements: its waits cost registers it has not)
   constexpr int lds = 2 * K * V * ln_bwd_threads(V, TPR, K) * (int)sizeof(float);
-  const int resident = ln_resident<kernel>(threads, lds), most = norm_max_slabs(a.M, a.F);
+  const int rows = ln_bwd_threads(V, TPR, K) / a.row, threads = rows * a.row, resident = ln_resident<kernel>(threads, lds);
+  // Streamed fp32 tables of short rows in order, as the forward takes them, two turns a workgroup and a slab for each:
+  // 10 M x 64 1.41 -> 1.22 ms (joined, and in 16 bits, nothing is gained: more arithmetic a byte).  From 32 rows a slab on
+  // the slabs are 2 % of the traffic.
+  constexpr int turns = 2;
+  if (NT && !JOIN && d.ws && norm_folds(a.M, a.F, sizeof(T)) && rows * turns >= NORM_FOLD_ROWS) {
+    const int blocks = (int)((a.M + rows * turns - 1) / (rows * turns)), folded = norm_blocks(blocks, 1, 256);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), lds, st, a, Walk{0, (int64_t)rows * turns, rows, turns}, d);
+    const int per = (blocks + folded - 1) / folded;
+    float *out = d.ws + (int64_t)blocks * 2 * a.F;
+    hipLaunchKernelGGL(ln_fold_k, dim3((unsigned)((2 * a.F + 63) / 64), folded), dim3(1024), 0, st, d.ws, blocks, per, a.F, out);
+    hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * a.F + 15) / 16)), dim3(1024), 0, st, out, folded, a.F, a.wdtype, d.gw, d.gb);
+    return 0;
+  }
   // (of the large tables sixteen waves a compute unit keep the memory busy; 24 of them were slower: 1.49 against 1.41 ms)
-  const int held = NT && resident > 512 ? 512 : resident;
+  const int most = norm_max_slabs(a.M, a.F), held = NT && resident > 512 ? 512 : resident;
   const int slabs = norm_blocks(a.M, rows, held < most ? held : most);
-  hipLaunchKernelGGL(kernel, dim3(slabs), dim3(threads), lds, st, a, d);
-  return slabs;
+  const int64_t step = (int64_t)slabs * rows;
+  hipLaunchKernelGGL(kernel, dim3(slabs), dim3(threads), lds, st, a, Walk{0, rows, step, (int)((a.M + step - 1) / step)}, d);
+  return slabs > 1 ? slabs : 0;
 }
 
 // every form: CASE(kind, V, TPR, K); LINE: those of large plain tables only
@@ -730,7 +800,7 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
 template <typename T>
 int ln_fwd(const NormFwd &n, hipStream_t st) {
   constexpr int V = Tab<T>::V;
-  const bool join = n.res || n.d.p > 0.f || n.sum, nt = streams(n.M * n.F, sizeof(T)) && whole_lines(n.F, sizeof(T));
+  const bool join = n.res || n.d.p > 0.f || n.sum, nt = norm_streams(n.M, n.F, sizeof(T));
   const NormForm f = norm_form(n.F, V, nt && !join);
   const Ln<T> a{(const T *)n.x, (const T *)n.res, n.w, n.b, n.M, (int)n.F, n.wdtype, f.row, n.d};
   T *y = (T *)n.y, *sum = (T *)n.sum;
@@ -763,7 +833,7 @@ int ln_fwd(const NormFwd &n, hipStream_t st) {
 template <typename T>
 int ln_bwd(const NormBwd &n, hipStream_t st) {
   constexpr int V = Tab<T>::V;
-  const bool join = n.res || n.d.p > 0.f || n.gsum || n.gres, nt = streams(n.M * n.F, sizeof(T)) && whole_lines(n.F, sizeof(T));
+  const bool join = n.res || n.d.p > 0.f || n.gsum || n.gres, nt = norm_streams(n.M, n.F, sizeof(T));
   const NormForm f = norm_form(n.F, V, nt && !join);
   const Ln<T> a{(const T *)n.x, (const T *)n.res, n.w, nullptr, n.M, (int)n.F, n.wdtype, f.row, n.d};
   const Grads<T> d{(const T *)n.g, (const T *)n.gsum, n.mean, n.rstd, (T *)n.gx, (T *)n.gres,
@@ -795,7 +865,7 @@ int ln_bwd(const NormBwd &n, hipStream_t st) {
 #undef LINE
     GSAGE_CHECK_LAUNCH();
   }
-  if (d.ws && (slabs != 1 || f.kind == NORM_LONG)) {
+  if (d.ws && (slabs > 0 || n.M == 0)) {
     hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * n.F + 15) / 16)), dim3(1024), 0, st, d.ws, slabs, (int)n.F, n.wdtype,
                        d.gw, d.gb);
     GSAGE_CHECK_LAUNCH();
@@ -804,10 +874,14 @@ int ln_bwd(const NormBwd &n, hipStream_t st) {
 }
 
 template <typename T> int dropout_go(const void *x, int64_t n, const NormDrop &d, void *out, hipStream_t st) {
-  const dim3 grid(gs_grid(n, 256 * 16)), block(256);
-  if (streams(n, sizeof(T))) hipLaunchKernelGGL((dropout_k<T, true>), grid, block, 0, st, (const T *)x, n, d, (T *)out);
-  else hipLaunchKernelGGL((dropout_k<T, false>), grid, block, 0, st, (const T *)x, n, d, (T *)out);
-  GSAGE_CHECK_LAUNCH();
+  const int64_t threads = n / Tab<T>::V + n % Tab<T>::V;
+  for (int64_t begin = 0; begin < threads; begin += (int64_t)MAX_GRID * 256) {
+    const int64_t left = (threads - begin + 255) / 256;
+    const dim3 grid((unsigned)(left < MAX_GRID ? left : MAX_GRID)), block(256);
+    if (norm_large(n, sizeof(T))) hipLaunchKernelGGL((dropout_k<T, true>), grid, block, 0, st, (const T *)x, n, begin, d, (T *)out);
+    else hipLaunchKernelGGL((dropout_k<T, false>), grid, block, 0, st, (const T *)x, n, begin, d, (T *)out);
+    GSAGE_CHECK_LAUNCH();
+  }
   return GSAGE_OK;
 }
 

@@ -416,3 +416,58 @@ def test_joined_past_2_to_the_32_elements():
         want = ref.reference(x.detach()[part].cpu(), weight=w.cpu(), p=p, seed=seed, g=g[part].cpu(), first=r0 * F)
         ref.check(y[part], want["y"], f"rows from {r0}")
         ref.check(dx[part], want["grad_x"], f"rows from {r0}")
+
+
+@pytest.mark.parametrize("M,F,dtype,joined", [
+    (1_050_011, 64, torch.float32, False), (1_050_011, 64, torch.float32, True), (524_301, 128, torch.float32, False),
+    (524_301, 128, torch.float32, True), (262_151, 256, torch.float32, False), (2_100_001, 64, torch.bfloat16, False),
+    (2_100_001, 64, torch.float16, True), (1_050_011, 128, torch.bfloat16, False), (525_001, 256, torch.float16, False),
+    (262_151, 512, torch.bfloat16, False), (350_003, 384, torch.bfloat16, True), (131_101, 1024, torch.bfloat16, True),
+    (66_001, 2048, torch.float16, False), (33_001, 2048, torch.float32, True), (16_800, 8192, torch.bfloat16, False)])
+def test_tables_beyond_the_caches(M, F, dtype, joined):
+    """From 256 MB on whole-line tables take the streaming forms: sampled rows against the formulas, the column sums
+    against sums over the whole table in float64 on the GPU."""
+    p, seed = (0.3, 77) if joined else (0.0, 0)
+    gen = torch.Generator(device="cuda").manual_seed(F)
+
+    def rnd(*size):
+        return torch.empty(*size, dtype=dtype, device="cuda").normal_(generator=gen)
+    x, g = rnd(M, F).requires_grad_(), rnd(M, F)
+    res = rnd(M, F).requires_grad_() if joined else None
+    w = (1 + 0.1 * rnd(F).float()).requires_grad_()
+    b = rnd(F).float().requires_grad_()
+    y = gs.dropout_add_layer_norm(x, res, w, b, p=p, seed=seed)
+    leaves = [t for t in (x, res, w, b) if t is not None]
+    grads = torch.autograd.grad(y, leaves, g)
+    names = ["grad_x"] + (["grad_residual"] if joined else [])
+    for r0 in (0, 17, M // 2 - 3, M - 13):
+        part = slice(r0, r0 + 13)
+        want = ref.reference(x.detach()[part].cpu(), res.detach()[part].cpu() if joined else None, w.detach().cpu(),
+                             b.detach().cpu(), p=p, seed=seed, g=g[part].cpu(), first=r0 * F)
+        ref.check(y[part], want["y"], f"rows from {r0}")
+        for name, got in zip(names, grads):
+            ref.check(got[part], want[name], f"rows from {r0} {name}")
+    # h from y: (y - b) / w, off by y's bound over w >= 0.5 and y's rounding; g h summed over the rows
+    dw = torch.zeros(F, dtype=torch.float64, device="cuda")
+    size = torch.zeros(F, dtype=torch.float64, device="cuda")
+    for r0 in range(0, M, 1 << 18):
+        part = slice(r0, r0 + (1 << 18))
+        gd = g[part].double()
+        h = (y.detach()[part].double() - b.detach().double()) / w.detach().double()
+        dw += (gd * h).sum(0)
+        size += (gd.abs() * (h.abs() + 3)).sum(0)
+    # every term: y's rounding (half a step of |w h + b| <= 2 (|h| + 3) over |w| >= 0.5: a factor 4), the bounds of h
+    # (H <= 100 u (|h| + 3) for rows of unit spread) and the sum's (64 + M / 64 roundings at most)
+    tol = (4 * ref.half_step(dtype) + 100 * ref.U + (66 + M / 64) * ref.U) * size
+    assert bool(((grads[-2].double() - dw).abs() <= tol).all())
+    db = g.sum(0, dtype=torch.float64)
+    assert bool(((grads[-1].double() - db).abs() <= (66 + M / 64) * ref.U * g.abs().sum(0, dtype=torch.float64)).all())
+
+
+def test_more_workgroups_than_one_launch_takes():
+    """17 M rows of 64: the forward's workgroups are dealt to more than one launch."""
+    M, F = (1 << 24) + 77, 64
+    x = torch.empty(M, F, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(4))
+    y = gs.layer_norm(x)
+    for r0 in (0, (1 << 23) - 5, (1 << 24) - 5, M - 10):
+        ref.check(y[r0:r0 + 10], ref.reference(x[r0:r0 + 10].cpu())["y"], f"rows from {r0}")
