@@ -151,5 +151,6 @@ def ptr(t) -> Optional[int]:
 
 
 def stream_handle() -> int:
+    """The current device's current stream (as torch.cuda.current_stream().cuda_stream, without building the object)."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())

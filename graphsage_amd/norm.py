@@ -20,8 +20,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .ops import _bracket
+from . import _lib, ops
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _M64 = (1 << 64) - 1
@@ -37,18 +36,14 @@ def _table(t: torch.Tensor, name: str) -> torch.Tensor:
     return t.contiguous()
 
 
-def _like(t: Optional[torch.Tensor], x: torch.Tensor, name: str) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
+def _like(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
     if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
         raise ValueError(f"{name} must have the input's shape, type and device ({tuple(x.shape)}, {x.dtype}, {x.device}), "
                          f"got {tuple(t.shape)}, {t.dtype}, {t.device}")
     return t.contiguous()
 
 
-def _affine(t: Optional[torch.Tensor], x: torch.Tensor, name: str) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
+def _affine(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
     if t.device != x.device:
         raise ValueError(f"{name} must live on the input's device {x.device}, got {t.device}")
     if t.dim() != 1 or t.numel() != x.size(-1):
@@ -86,67 +81,93 @@ def _split(seed) -> Tuple[int, Optional[int]]:
 
 
 # ----------------------------------------------------------------------------------------------- raw ops
+def _call(tag: str, device: torch.device, entry, *args) -> None:
+    """``entry(*args, stream)`` on ``device``'s current stream.  Allocations belong to a device whichever is current;
+    the launch does not."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(tag, device, entry, *args)
+    if ops._timer is None:
+        status = entry(*args, _lib.stream_handle())
+    else:
+        with ops._bracket(tag):
+            status = entry(*args, _lib.stream_handle())
+    if status:
+        _lib.check(status, "gsage_" + tag)
+
+
 def _dropout(x: torch.Tensor, p: float, seed) -> torch.Tensor:
     value, pointer = _split(seed)
-    with torch.cuda.device(x.device):
-        out = torch.empty_like(x)
-        with _bracket("dropout"):
-            rc = _lib.load().gsage_dropout(x.data_ptr(), x.numel(), _DTYPES[x.dtype], p, value, pointer, out.data_ptr(),
-                                           _lib.stream_handle())
-    _lib.check(rc, "gsage_dropout")
+    out = torch.empty_like(x)
+    _call("dropout", x.device, _lib.load().gsage_dropout, x.data_ptr(), x.numel(), _DTYPES[x.dtype], p, value, pointer,
+          out.data_ptr())
     return out
 
 
-def _wdtype(weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], x: torch.Tensor) -> int:
-    t = weight if weight is not None else bias
-    return _DTYPES[x.dtype if t is None else t.dtype]
-
-
 def layer_norm_fwd(x, residual, weight, bias, eps: float, p: float, seed, want_sum: bool, want_stats: bool):
-    """gsage_layer_norm_fwd on contiguous operands -> (y, sum or None, mean or None, rstd or None)."""
+    """gsage_layer_norm_fwd on contiguous operands -> (y, sum or None, [mean, rstd] as fp32 [2, M] or None)."""
     value, pointer = _split(seed)
     F = x.size(-1)
     M = x.numel() // F
-    with torch.cuda.device(x.device):
-        y = torch.empty_like(x)
-        total = torch.empty_like(x) if want_sum else None
-        mean = rstd = None
-        if want_stats:
-            mean, rstd = torch.empty(2, M, dtype=torch.float32, device=x.device).unbind(0)
-        with _bracket("layer_norm_fwd"):
-            rc = _lib.load().gsage_layer_norm_fwd(
-                x.data_ptr(), _lib.ptr(residual), _lib.ptr(weight), _lib.ptr(bias), M, F, _DTYPES[x.dtype],
-                _wdtype(weight, bias, x), eps, p, value, pointer, y.data_ptr(), _lib.ptr(total), _lib.ptr(mean),
-                _lib.ptr(rstd), _lib.stream_handle())
-    _lib.check(rc, "gsage_layer_norm_fwd")
-    return y, total, mean, rstd
+    y = torch.empty_like(x)
+    total = torch.empty_like(x) if want_sum else None
+    stats = mean = rstd = None
+    if want_stats:
+        stats = torch.empty((2, M), dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * M
+    code = _DTYPES[x.dtype]
+    affine = weight if weight is not None else bias
+    _call("layer_norm_fwd", x.device, _lib.load().gsage_layer_norm_fwd, x.data_ptr(), _lib.ptr(residual),
+          _lib.ptr(weight), _lib.ptr(bias), M, F, code, code if affine is None else _DTYPES[affine.dtype], eps, p, value,
+          pointer, y.data_ptr(), _lib.ptr(total), mean, rstd)
+    return y, total, stats
 
 
-def layer_norm_bwd(grad_y, grad_sum, x, residual, weight, mean, rstd, p: float, seed, need, wdtype: torch.dtype):
+def layer_norm_bwd(grad_y, grad_sum, x, residual, weight, stats, p: float, seed, need, wdtype: torch.dtype):
     """gsage_layer_norm_bwd -> (grad_x, grad_residual, grad_weight, grad_bias), None where ``need`` is false."""
     lib = _lib.load()
     value, pointer = _split(seed)
+    dev, code = x.device, _DTYPES[x.dtype]
     F = x.size(-1)
     M = x.numel() // F
-    with torch.cuda.device(x.device):
-        gx = torch.empty_like(x) if need[0] else None
-        gres = torch.empty_like(x) if need[1] else None
-        gw = torch.empty(F, dtype=wdtype, device=x.device) if need[2] else None
-        gb = torch.empty(F, dtype=wdtype, device=x.device) if need[3] else None
-        ws, ws_bytes = None, 0
-        if need[2] or need[3]:
-            ws_bytes = lib.gsage_layer_norm_bwd_workspace_bytes(M, F, _DTYPES[x.dtype])
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-        with _bracket("layer_norm_bwd"):
-            rc = lib.gsage_layer_norm_bwd(
-                grad_y.data_ptr(), _lib.ptr(grad_sum), x.data_ptr(), _lib.ptr(residual), _lib.ptr(weight),
-                mean.data_ptr(), rstd.data_ptr(), M, F, _DTYPES[x.dtype], _DTYPES[wdtype], p, value, pointer,
-                _lib.ptr(gx), _lib.ptr(gres), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws), ws_bytes, _lib.stream_handle())
-    _lib.check(rc, "gsage_layer_norm_bwd")
+    gx = torch.empty_like(x) if need[0] else None
+    gres = torch.empty_like(x) if need[1] else None
+    gw = torch.empty(F, dtype=wdtype, device=dev) if need[2] else None
+    gb = torch.empty(F, dtype=wdtype, device=dev) if need[3] else None
+    ws, ws_bytes = None, 0
+    if need[2] or need[3]:
+        ws_bytes = lib.gsage_layer_norm_bwd_workspace_bytes(M, F, code)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    mean = stats.data_ptr()
+    _call("layer_norm_bwd", dev, lib.gsage_layer_norm_bwd, grad_y.data_ptr(), _lib.ptr(grad_sum), x.data_ptr(),
+          _lib.ptr(residual), _lib.ptr(weight), mean, mean + 4 * M, M, F, code, _DTYPES[wdtype], p, value, pointer,
+          _lib.ptr(gx), _lib.ptr(gres), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws), ws_bytes)
     return gx, gres, gw, gb
 
 
 # ----------------------------------------------------------------------------------------- autograd glue
+def _keep_seed(ctx, seed, *tensors) -> None:
+    # a seed tensor is saved like any operand: rewriting it between forward and backward is an error,
+    # not another mask
+    if torch.is_tensor(seed):
+        ctx.seed = None
+        ctx.save_for_backward(*tensors, seed)
+    else:
+        ctx.seed = seed
+        ctx.save_for_backward(*tensors)
+
+
+def _once(backward):
+    """A backward of raw kernels: not differentiable again.  torch's own wrapper for that only where a graph of the
+    backward is wanted (it costs as much as a launch)."""
+    refusing = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p: float, seed):
@@ -155,20 +176,10 @@ class DropoutFunction(torch.autograd.Function):
         return _dropout(x, p, seed)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out):
-        return _dropout(grad_out.contiguous(), ctx.p, _kept_seed(ctx, ctx.saved_tensors)), None, None
-
-
-def _keep_seed(ctx, seed, *tensors) -> None:
-    # a seed tensor is saved like any operand: rewriting it between forward and backward is an error,
-    # not another mask
-    ctx.seed = None if torch.is_tensor(seed) else seed
-    ctx.save_for_backward(*tensors, *((seed,) if ctx.seed is None else ()))
-
-
-def _kept_seed(ctx, saved):
-    return saved[-1] if ctx.seed is None else ctx.seed
+        seed = ctx.seed if ctx.seed is not None else ctx.saved_tensors[0]
+        return _dropout(grad_out.contiguous(), ctx.p, seed), None, None
 
 
 class LayerNormFunction(torch.autograd.Function):
@@ -176,23 +187,26 @@ class LayerNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps: float, p: float, seed, return_sum: bool):
-        y, total, mean, rstd = layer_norm_fwd(x, residual, weight, bias, eps, p, seed, return_sum, True)
+        y, total, stats = layer_norm_fwd(x, residual, weight, bias, eps, p, seed, return_sum, True)
         ctx.p = p
-        ctx.wdtype = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
-        _keep_seed(ctx, seed, x, residual, weight, mean, rstd)
+        affine = weight if weight is not None else bias
+        ctx.wdtype = torch.float32 if affine is None else affine.dtype
+        _keep_seed(ctx, seed, x, residual, weight, stats)
         ctx.set_materialize_grads(False)
         return (y, total) if return_sum else y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y, grad_sum=None):
         if grad_y is None and grad_sum is None:
             return (None,) * 8
-        x, residual, weight, mean, rstd = ctx.saved_tensors[:5]
+        saved = ctx.saved_tensors
+        x, residual, weight, stats = saved[:4]
         grad_y = torch.zeros_like(x) if grad_y is None else grad_y.contiguous()
-        grad_sum = None if grad_sum is None else grad_sum.contiguous()
-        grads = layer_norm_bwd(grad_y, grad_sum, x, residual, weight, mean, rstd, ctx.p,
-                               _kept_seed(ctx, ctx.saved_tensors), ctx.needs_input_grad[:4], ctx.wdtype)
+        if grad_sum is not None:
+            grad_sum = grad_sum.contiguous()
+        grads = layer_norm_bwd(grad_y, grad_sum, x, residual, weight, stats, ctx.p,
+                               ctx.seed if ctx.seed is not None else saved[4], ctx.needs_input_grad, ctx.wdtype)
         return (*grads, None, None, None, None)
 
 
@@ -228,16 +242,22 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
     x = _table(x, "x")
     if x.dim() == 0 or x.size(-1) == 0:
         raise ValueError(f"layer norm needs at least one column, got x of shape {tuple(x.shape)}")
-    residual = _like(residual, x, "residual")
-    weight, bias = _affine(weight, x, "weight"), _affine(bias, x, "bias")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
+    if residual is not None:
+        residual = _like(residual, x, "residual")
+    if weight is not None:
+        weight = _affine(weight, x, "weight")
+    if bias is not None:
+        bias = _affine(bias, x, "bias")
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
     if not training:
         p = 0.0
     seed = _seed(seed, x.device) if p > 0.0 else 0
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad) or
+                                    (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
         return LayerNormFunction.apply(x, residual, weight, bias, eps, p, seed, return_sum)
-    y, total, _, _ = layer_norm_fwd(x, residual, weight, bias, eps, p, seed, return_sum, False)
+    y, total, _ = layer_norm_fwd(x, residual, weight, bias, eps, p, seed, return_sum, False)
     return (y, total) if return_sum else y
 
 
