@@ -13,7 +13,7 @@ from typing import Dict, Optional
 
 import torch
 
-from .graphsage import GraphSAGE
+from .graphsage import GraphSAGE, depth_options
 
 
 def model_from_checkpoint(checkpoint: dict, fallback_config: Optional[dict] = None) -> GraphSAGE:
@@ -21,7 +21,7 @@ def model_from_checkpoint(checkpoint: dict, fallback_config: Optional[dict] = No
     mc, fc = cfg.get("model", {}), cfg.get("features", {})
     model = GraphSAGE(in_channels=fc.get("dimensions", 7), hidden_channels=mc.get("hidden_dim", 64),
                       out_channels=mc.get("output_dim", 64), num_layers=mc.get("num_layers", 2),
-                      dropout=0.0, normalize_output=mc.get("normalize_output", True))
+                      dropout=0.0, normalize_output=mc.get("normalize_output", True), **depth_options(mc))
     model.load_state_dict(checkpoint["model_state_dict"])      # strict, PyG key layout
     return model
 

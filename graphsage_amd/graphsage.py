@@ -18,6 +18,7 @@ import torch.nn.functional as F
 from . import _lib
 from .graph import GraphCSR, default_cache
 from . import ops
+from .norm import LayerNorm, dropout, dropout_add_layer_norm
 from .ops import SAGELayerFunction, aggregate_mean
 
 
@@ -38,6 +39,7 @@ def vector_width(f: int) -> int:
 
 
 _M64 = (1 << 64) - 1
+INPUT_SLOT = 63       # mix_seed's layer number of the input features' dropout
 
 
 def mix_seed(base: int, step: int, layer: int = 0) -> int:
@@ -114,12 +116,24 @@ class GraphSAGE(nn.Module):
 
     def __init__(self, in_channels: int = 7, hidden_channels: int = 64, out_channels: int = 64,
                  num_layers: int = 2, dropout: float = 0.3, aggregator: str = "mean",
-                 normalize_output: bool = True, cache_input_aggregation: bool = False):
+                 normalize_output: bool = True, cache_input_aggregation: bool = False,
+                 norm: Optional[str] = None, residual: bool = False, input_dropout: float = 0.0):
         """``cache_input_aggregation`` (not in the reference): keep the first layer's
         ``mean_j x_j`` between calls while the feature tensor and the graph are unchanged, as
         they are across training steps.  Same results; off by default because the reference
-        recomputes it, and so does the benchmark."""
+        recomputes it, and so does the benchmark.
+
+        For deeper encoders (what the reference's FlexibleGraphSAGE, ``:160-296``, tries out):
+        ``norm="layer"``: hidden layer i is ``LayerNorm(dropout(relu(conv_i(h))))`` (parameters
+        ``norms.{i}.weight / .bias``), with ``residual=True`` ``LayerNorm(h + dropout(relu(conv_i(h))))``
+        from the second on.  ``input_dropout``: dropout of the features while training."""
         super().__init__()
+        if norm not in (None, "layer"):
+            raise ValueError(f"Unknown norm: {norm!r} (None or 'layer')")
+        if residual and norm is None:
+            raise ValueError("residual=True is part of norm='layer'")
+        if not 0.0 <= float(input_dropout) < 1.0:
+            raise ValueError(f"input_dropout must be in [0, 1), got {input_dropout}")
         self.in_channels = in_channels
         self.hidden_channels = hidden_channels
         self.out_channels = out_channels
@@ -133,6 +147,9 @@ class GraphSAGE(nn.Module):
             self.convs.append(SAGEConv(hidden_channels, hidden_channels, aggr=aggregator))
         if num_layers > 1:
             self.convs.append(SAGEConv(hidden_channels, out_channels, aggr=aggregator))
+        self.norm, self.residual, self.input_dropout = norm, bool(residual), float(input_dropout)
+        if norm is not None:
+            self.norms = nn.ModuleList([LayerNorm(hidden_channels) for _ in self.convs[:-1]])
         # kept for API parity (reference attribute `dropout`); the mask itself is drawn
         # inside the K3 epilogue, not by this module
         self.dropout = nn.Dropout(dropout)
@@ -157,13 +174,26 @@ class GraphSAGE(nn.Module):
         return int(torch.empty((), dtype=torch.int64).random_().item())
 
     def forward(self, x: torch.Tensor, edge_index: torch.Tensor,
-                keep_masks: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+                keep_masks: Optional[Sequence[torch.Tensor]] = None,
+                dropout_seeds: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x: fp32 [N, in_channels]; edge_index: int64 [2, E] -> fp32 [N, out_channels].
 
         ``keep_masks`` (optional, one uint8 [N, hidden] tensor per hidden layer) injects the
-        dropout masks instead of drawing them in the kernel (parity tests).
+        dropout masks instead of drawing them in the kernel (parity tests; not with ``norm``).
+        ``dropout_seeds`` (optional, int64 [num_layers] on the device: the hidden layers' seeds, then
+        ``input_dropout``'s) seeds the masks of ``norm`` and ``input_dropout`` from memory, for a
+        captured graph that rewrites it.
         """
         graph = default_cache().get(edge_index, x.size(0))
+        if dropout_seeds is not None and dropout_seeds.numel() != len(self.convs):
+            raise ValueError(f"dropout_seeds must hold {len(self.convs)} seeds, got {tuple(dropout_seeds.shape)}")
+        dropped = self.training and self.input_dropout > 0.0
+        if dropped:
+            x = dropout(x, self.input_dropout, seed=self._layer_seed(INPUT_SLOT, dropout_seeds, len(self.convs) - 1))
+        if self.norm is not None:
+            if keep_masks is not None:
+                raise ValueError("keep_masks are not taken with norm='layer': its masks are drawn in the kernel")
+            return self._forward_normed(x, graph, dropout_seeds, not dropped)
         if self._blocked_inference_applies(x):
             return self._forward_blocked(x, graph)
         p = float(self.dropout_rate)
@@ -198,17 +228,38 @@ class GraphSAGE(nn.Module):
                 km = keep_masks[i] if keep_masks is not None else None
                 seed = 0 if km is not None else self._dropout_seed(i)
                 x = conv.run(x, graph, _lib.EPI_RELU_DROPOUT, p, seed, km, self._force_generic,
-                             input_layer=i == 0, agg=agg_for(i), stash=stash if i == 0 else None,
+                             input_layer=i == 0 and not dropped, agg=agg_for(i), stash=stash if i == 0 else None,
                              amax_in=a_in, amax_out=a_out, upstream=upstream_of(i))
             else:
                 x = conv.run(x, graph, _lib.EPI_RELU, 0.0, 0, None, self._force_generic,
-                             input_layer=i == 0, agg=agg_for(i), stash=stash if i == 0 else None,
+                             input_layer=i == 0 and not dropped, agg=agg_for(i), stash=stash if i == 0 else None,
                              amax_in=a_in, amax_out=a_out)
         epi = _lib.EPI_L2NORM if self.normalize_output else _lib.EPI_NONE
         last = len(self.convs) - 1
         return self.convs[-1].run(x, graph, epi, 0.0, 0, None, self._force_generic,
-                                  input_layer=last == 0, agg=agg_for(last), amax_in=amax_of(last)[0],
+                                  input_layer=last == 0 and not dropped, agg=agg_for(last),
+                                  amax_in=amax_of(last)[0],
                                   upstream=upstream_of(last))
+
+    def _layer_seed(self, slot: int, dropout_seeds: Optional[torch.Tensor], at: int):
+        return self._dropout_seed(slot) if dropout_seeds is None else dropout_seeds.view(-1)[at]
+
+    def _forward_normed(self, x: torch.Tensor, graph: GraphCSR, dropout_seeds: Optional[torch.Tensor],
+                        input_is_constant: bool) -> torch.Tensor:
+        """``norm="layer"``: each hidden layer's ReLU in its projection; dropout, residual and norm in
+        one pass behind it.  (What the plain path hands from layer to layer -- operands for the
+        recomputed aggregation, ranges -- describes the projection's output, which is not what the
+        next layer reads here.)"""
+        p = float(self.dropout_rate) if self.training else 0.0
+        for i, (conv, norm) in enumerate(zip(self.convs[:-1], self.norms)):
+            r = conv.run(x, graph, _lib.EPI_RELU, force_generic=self._force_generic,
+                         input_layer=i == 0 and input_is_constant)
+            seed = self._layer_seed(i, dropout_seeds, i) if p > 0.0 else None
+            x = dropout_add_layer_norm(r, x if self.residual and i > 0 else None, norm.weight, norm.bias, p=p,
+                                       eps=norm.eps, seed=seed)
+        epi = _lib.EPI_L2NORM if self.normalize_output else _lib.EPI_NONE
+        return self.convs[-1].run(x, graph, epi, force_generic=self._force_generic,
+                                  input_layer=len(self.convs) == 1 and input_is_constant)
 
     def _range_words(self, x: torch.Tensor) -> Optional[torch.Tensor]:
         """One int32 word per hidden layer for max |activation| (float bits), when every layer can
@@ -291,9 +342,16 @@ class GraphSAGE(nn.Module):
     def reset_parameters(self) -> None:
         for conv in self.convs:
             conv.reset_parameters()
+        for norm in (self.norms if self.norm is not None else ()):
+            norm.reset_parameters()
 
     def count_parameters(self) -> int:
         return sum(p.numel() for p in self.parameters() if p.requires_grad)
+
+
+def depth_options(model_cfg: dict) -> dict:
+    """The constructor's ``norm``, ``residual`` and ``input_dropout`` from a config's model section."""
+    return {k: model_cfg[k] for k in ("norm", "residual", "input_dropout") if k in model_cfg}
 
 
 def create_model(config: dict, device: Optional[torch.device] = None) -> GraphSAGE:
@@ -308,6 +366,7 @@ def create_model(config: dict, device: Optional[torch.device] = None) -> GraphSA
         dropout=model_cfg.get("dropout", 0.3),
         aggregator=model_cfg.get("aggregator", "mean"),
         normalize_output=model_cfg.get("normalize_output", True),
+        **depth_options(model_cfg),
     )
     if device is not None:
         model = model.to(device)

@@ -53,6 +53,8 @@ def receptive_forward(model, x: torch.Tensor, graph: GraphCSR, targets: torch.Te
     remapped into T).  2-layer models only."""
     if len(model.convs) != 2:
         raise ValueError("the receptive-field step covers 2-layer models")
+    if model.norm is not None or model.input_dropout > 0.0:
+        raise ValueError("the receptive-field step covers models without norm and input_dropout")
     B = targets.numel()
     ids = torch.cat([targets, contexts, negatives.reshape(-1)])
     if B and (int(ids.min()) < 0 or int(ids.max()) >= graph.num_nodes):   # the ids index the CSR here

@@ -243,12 +243,18 @@ class TrainStep:
         self.flat.zero_grad()
         masks = None
         p = float(getattr(model, "dropout_rate", 0.0))
-        if p > 0.0:
+        normed = getattr(model, "norm", None) is not None
+        if p > 0.0 and not normed:
             n = self.features.size(0)
             masks = [(torch.rand(n, conv.out_channels, device=self.features.device,
                                  generator=self._mask_gen) >= p).to(torch.uint8)
                      for conv in model.convs[:-1]]
-        emb = model(self.features, self.edge_index, keep_masks=masks)
+        more = {}
+        if (normed and p > 0.0) or getattr(model, "input_dropout", 0.0) > 0.0:
+            # masks drawn in the kernels, from seeds that the graph rewrites on each replay
+            more["dropout_seeds"] = torch.empty(len(model.convs), dtype=torch.int64,
+                                                device=self.features.device).random_(generator=self._mask_gen)
+        emb = model(self.features, self.edge_index, keep_masks=masks, **more)
         loss, stats = self.loss_fn.forward_stats(emb, self._gt, self._gc, self._gn,
                                                  global_batch=batch_size * self.world)
         loss.backward()

@@ -356,7 +356,7 @@ def train_graphsage(dataset, walks, config: Dict[str, Any], device=None):
     ``(features, edge_index)`` pair.  ``walks``: the reference's list of lists, or the
     ``(walks, lengths)`` tensors of :class:`RandomWalkGenerator`; the pairs are extracted on the
     device in the reference's order either way."""
-    from .graphsage import GraphSAGE
+    from .graphsage import GraphSAGE, depth_options
     from .sampler import DegreeBiasedNegativeSampler
     from .walks import CooccurrencePairSampler
     device = torch.device(device) if device is not None else torch.device("cuda")
@@ -384,7 +384,7 @@ def train_graphsage(dataset, walks, config: Dict[str, Any], device=None):
     model = GraphSAGE(in_channels=config.get("features", {}).get("dimensions", 7),
                       hidden_channels=mc.get("hidden_dim", 64), out_channels=mc.get("output_dim", 64),
                       num_layers=mc.get("num_layers", 2), dropout=mc.get("dropout", 0.3),
-                      normalize_output=mc.get("normalize_output", True)).to(device)
+                      normalize_output=mc.get("normalize_output", True), **depth_options(mc)).to(device)
     trainer = GraphSAGETrainer(model, features, edge_index, pairs, neg_sampler, config)
     trainer.train(num_epochs=config.get("training", {}).get("epochs", 100))
     return model, trainer.get_embeddings()

@@ -91,3 +91,24 @@ def test_mask_of_a_long_table_counts_in_64_bits():
     first = (1 << 32) - 3
     part = rng.dropout_keep_mask_range(99, first, 8, 0.5)
     assert (part[3:] != rng.dropout_keep_mask_range(99, 0, 5, 0.5)).any()      # not the first elements' again
+
+
+def test_model_options():
+    from graphsage_amd import GraphSAGE, create_model
+    m = GraphSAGE(num_layers=3, norm="layer", residual=True)
+    assert [k for k in m.state_dict() if k.startswith("norms")] == ["norms.0.weight", "norms.0.bias", "norms.1.weight",
+                                                                   "norms.1.bias"]
+    assert not any(k.startswith("norms") for k in GraphSAGE().state_dict())
+    assert len(GraphSAGE(num_layers=1, norm="layer").norms) == 0
+    for bad in (dict(norm="batch"), dict(residual=True), dict(input_dropout=1.0), dict(input_dropout=-0.1)):
+        with pytest.raises(ValueError):
+            GraphSAGE(**bad)
+    cfg = {"model": {"num_layers": 3, "norm": "layer", "residual": True, "input_dropout": 0.25}}
+    m = create_model(cfg)
+    assert (m.norm, m.residual, m.input_dropout) == ("layer", True, 0.25)
+    with torch.no_grad():
+        m.norms[1].weight.zero_()
+    m.reset_parameters()
+    assert bool((m.norms[1].weight == 1).all())
+    with pytest.raises(ValueError, match="GPU"):
+        m.train()(torch.randn(5, 7), torch.zeros(2, 3, dtype=torch.int64))
