@@ -92,11 +92,11 @@ SIGNATURES = {
     "gsage_skipgram_fwd_noalloc": (C.c_int, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, C.c_float,
                                              C.c_double, C.c_double, _p, _p, _p]),
     "gsage_skipgram_bwd": (C.c_int, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _p, _p]),
-    "gsage_dropout": (C.c_int, [_p, _i64, C.c_int, C.c_float, C.c_uint64, _p, _p, _p]),
-    "gsage_layer_norm_fwd": (C.c_int, [_p, _p, _p, _p, _i64, _i64, C.c_int, C.c_int, C.c_float, C.c_float,
+    "gsage_dropout": (C.c_int, [_p, _i64, C.c_int, C.c_double, C.c_uint64, _p, _p, _p]),
+    "gsage_layer_norm_fwd": (C.c_int, [_p, _p, _p, _p, _i64, _i64, C.c_int, C.c_int, C.c_float, C.c_double,
                                        C.c_uint64, _p, _p, _p, _p, _p, _p]),
     "gsage_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, C.c_int]),
-    "gsage_layer_norm_bwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, C.c_int, C.c_int, C.c_float,
+    "gsage_layer_norm_bwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, C.c_int, C.c_int, C.c_double,
                                        C.c_uint64, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "gsage_alias_build_host": (C.c_int, [_p, _i64, _p, _p]),
     "gsage_alias_sample": (C.c_int, [_p, _p, _i64, _i64, C.c_uint64, C.c_uint64, _p, _p]),

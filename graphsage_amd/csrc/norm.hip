@@ -8,22 +8,25 @@ constexpr int64_t MAX_F = 1 << 24;
 constexpr int64_t MAX_N = (int64_t)1 << 40;
 
 bool bad_dtype(int d) { return d != GSAGE_F32 && d != GSAGE_BF16 && d != GSAGE_F16; }
-bool bad_p(float p) { return !(p >= 0.f && p < 1.f); }
+// The mask counts the rate as the fp32 number that the projection's epilogue takes (so the masks are the same); the scale
+// is that of the rate as given: 1 - p of a rounded p is off by up to 2^-25 / (1 - p).
+bool bad_p(double p) { return !(p >= 0. && (float)p < 1.f); }
+NormDrop drop_of(double p, uint64_t seed, const int64_t *seed_dev) { return {(float)p, (float)(1. / (1. - p)), seed, seed_dev}; }
 
 }  // namespace
 
-extern "C" int gsage_dropout(const void *x, int64_t n, int dtype, float p, uint64_t seed, const int64_t *seed_dev,
+extern "C" int gsage_dropout(const void *x, int64_t n, int dtype, double p, uint64_t seed, const int64_t *seed_dev,
                              void *out, gsage_stream_t stream) {
   if (n < 0 || bad_dtype(dtype) || bad_p(p)) return GSAGE_ERR_INVALID_ARG;
   if (n == 0) return GSAGE_OK;
   if (!x || !out) return GSAGE_ERR_INVALID_ARG;
   if (n > MAX_N) return GSAGE_ERR_UNSUPPORTED;
   const auto go = dtype == GSAGE_F32 ? norm_dropout_f32 : dtype == GSAGE_BF16 ? norm_dropout_bf16 : norm_dropout_f16;
-  return go(x, n, NormDrop{p, 1.0f / (1.0f - p), seed, seed_dev}, out, gs_stream(stream));
+  return go(x, n, drop_of(p, seed, seed_dev), out, gs_stream(stream));
 }
 
 extern "C" int gsage_layer_norm_fwd(const void *x, const void *residual, const void *weight, const void *bias, int64_t M,
-                                    int64_t F, int dtype, int wdtype, float eps, float p, uint64_t seed,
+                                    int64_t F, int dtype, int wdtype, float eps, double p, uint64_t seed,
                                     const int64_t *seed_dev, void *y, void *sum, float *mean, float *rstd,
                                     gsage_stream_t stream) {
   if (M < 0 || F <= 0 || bad_dtype(dtype) || bad_p(p) || !(eps >= 0.f)) return GSAGE_ERR_INVALID_ARG;
@@ -33,7 +36,7 @@ extern "C" int gsage_layer_norm_fwd(const void *x, const void *residual, const v
   if (!x || !y) return GSAGE_ERR_INVALID_ARG;
   if (F > MAX_F || M > MAX_N / F) return GSAGE_ERR_UNSUPPORTED;
   const auto go = dtype == GSAGE_F32 ? norm_fwd_f32 : dtype == GSAGE_BF16 ? norm_fwd_bf16 : norm_fwd_f16;
-  return go(NormFwd{x, residual, weight, bias, M, F, wdtype, eps, {p, 1.0f / (1.0f - p), seed, seed_dev}, y, sum, mean, rstd},
+  return go(NormFwd{x, residual, weight, bias, M, F, wdtype, eps, drop_of(p, seed, seed_dev), y, sum, mean, rstd},
             gs_stream(stream));
 }
 
@@ -44,7 +47,7 @@ extern "C" size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int
 
 extern "C" int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, const void *x, const void *residual,
                                     const void *weight, const float *mean, const float *rstd, int64_t M, int64_t F,
-                                    int dtype, int wdtype, float p, uint64_t seed, const int64_t *seed_dev, void *grad_x,
+                                    int dtype, int wdtype, double p, uint64_t seed, const int64_t *seed_dev, void *grad_x,
                                     void *grad_residual, void *grad_weight, void *grad_bias, void *ws, size_t ws_bytes,
                                     gsage_stream_t stream) {
   if (M < 0 || F <= 0 || bad_dtype(dtype) || bad_p(p)) return GSAGE_ERR_INVALID_ARG;
@@ -56,7 +59,7 @@ extern "C" int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, co
     if (ws_bytes < gsage_layer_norm_bwd_workspace_bytes(M, F, dtype)) return GSAGE_ERR_WORKSPACE;
   }
   const auto go = dtype == GSAGE_F32 ? norm_bwd_f32 : dtype == GSAGE_BF16 ? norm_bwd_bf16 : norm_bwd_f16;
-  return go(NormBwd{grad_y, grad_sum, x, residual, weight, mean, rstd, M, F, wdtype, {p, 1.0f / (1.0f - p), seed, seed_dev},
+  return go(NormBwd{grad_y, grad_sum, x, residual, weight, mean, rstd, M, F, wdtype, drop_of(p, seed, seed_dev),
                     grad_x, grad_residual, grad_weight, grad_bias, (float *)ws},
             gs_stream(stream));
 }

@@ -558,20 +558,20 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
   flush();
   __syncthreads();
   // this workgroup's column sums -> its slab, or (one workgroup) the result: element e of thread t's columns, over the
-  // threads of the workgroup's rows that hold the same columns
+  // threads of the workgroup's rows that hold the same columns (up to 128: in double)
   float *slab = d.ws + (int64_t)blockIdx.x * 2 * a.F;
   for (int j = threadIdx.x; j < K * V * c.threads; j += blockDim.x) {
     const int t = j % c.threads, e = j / c.threads, v = (t + e / V * c.threads) * V, at = v < a.F - V ? v : a.F - V;
     if (v >= a.F || e % V < v - at) continue;
-    float u = 0.f, q = 0.f;
+    double u = 0., q = 0.;
     for (int r = 0; r < rows; ++r) {
       u += acc[e * threads + r * c.threads + t];
       q += acc[(K * V + e) * threads + r * c.threads + t];
     }
     const int col = at + e % V;
-    if (gridDim.x > 1) { slab[col] = u; slab[a.F + col] = q; continue; }
-    if (d.gw) store_w(d.gw, a.wdtype, col, u);
-    if (d.gb) store_w(d.gb, a.wdtype, col, q);
+    if (gridDim.x > 1) { slab[col] = (float)u; slab[a.F + col] = (float)q; continue; }
+    if (d.gw) store_w(d.gw, a.wdtype, col, (float)u);
+    if (d.gb) store_w(d.gb, a.wdtype, col, (float)q);
   }
 }
 
@@ -747,8 +747,9 @@ void ln_fwd_launch(const Ln<T> &a, int turns, float eps, T *y, T *sum, float *me
   }
 }
 
-// One turn a workgroup, where it has 3 KB of rows to spread its weights over; 16-bit rows without dropout or a residual
-// need two (less arithmetic a byte: 4 M x 64 bf16 0.165 against 0.191 ms), and so do rows of two or four waves.  Rows of
+// One turn a workgroup, where it has 3200 bytes of rows to spread its weights over (fp32 2 M x 28: 81 us, 83 as a loop of
+// two turns; 2 M x 20: 70 us, as a loop 60; 4 M x 4 59 and 41); 16-bit rows without dropout or a residual need two (less
+// arithmetic a byte: 4 M x 64 bf16 0.165 against 0.191 ms), and so do rows of two or four waves.  Rows of
 // three waves and of 32 elements a thread run as loops over the grid that the GPU holds (8191 x 5120 bf16 33 us, 36 in
 // order; 8192 x 16000 100 us, 108).
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
@@ -757,7 +758,7 @@ void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd
   constexpr bool thin = sizeof(T) == 2 && !JOIN;
   if constexpr (TPR == 0) ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, K == 2 ? 2 : 0, eps, y, sum, mean, rstd, st);
   else if constexpr (thin || K == 1) {
-    if (thin || bytes < 3072)
+    if (thin || bytes < 3200)
       ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, bytes < 4096 ? (int)((8191 + bytes) / bytes) : 2, eps, y, sum, mean, rstd, st);
     else if constexpr (!thin) ln_fwd_launch<T, V, TPR, K, JOIN, NT, false>(a, 1, eps, y, sum, mean, rstd, st);
   } else ln_fwd_launch<T, V, TPR, K, JOIN, NT, false>(a, 1, eps, y, sum, mean, rstd, st);

@@ -55,7 +55,7 @@ def _affine(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
 
 def _rate(p: float) -> float:
     p = float(p)
-    if not 0.0 <= p < 1.0:
+    if not 0.0 <= p < 1.0 - 2.0 ** -25:           # (an fp32 number below 1)
         raise ValueError(f"dropout rate must be in [0, 1), got {p}")
     return p
 

@@ -499,16 +499,16 @@ int gsage_skipgram_bwd_rows(const float *emb, int64_t N, int64_t D, const int64_
  *   grad_bias is wanted). */
 enum gsage_dtype { GSAGE_F32 = 0, GSAGE_BF16 = 1, GSAGE_F16 = 2 };
 
-int gsage_dropout(const void *x, int64_t n, int dtype, float p, uint64_t seed,
+int gsage_dropout(const void *x, int64_t n, int dtype, double p, uint64_t seed,
                   const int64_t *seed_dev, void *out, gsage_stream_t stream);
 int gsage_layer_norm_fwd(const void *x, const void *residual, const void *weight, const void *bias,
-                         int64_t M, int64_t F, int dtype, int wdtype, float eps, float p,
+                         int64_t M, int64_t F, int dtype, int wdtype, float eps, double p,
                          uint64_t seed, const int64_t *seed_dev, void *y, void *sum, float *mean,
                          float *rstd, gsage_stream_t stream);
 size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype);
 int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, const void *x,
                          const void *residual, const void *weight, const float *mean,
-                         const float *rstd, int64_t M, int64_t F, int dtype, int wdtype, float p,
+                         const float *rstd, int64_t M, int64_t F, int dtype, int wdtype, double p,
                          uint64_t seed, const int64_t *seed_dev, void *grad_x, void *grad_residual,
                          void *grad_weight, void *grad_bias, void *ws, size_t ws_bytes,
                          gsage_stream_t stream);

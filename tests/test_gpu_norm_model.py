@@ -206,8 +206,7 @@ def test_input_dropout_on_the_plain_model():
     m.train(), plain.train()
     m.set_dropout_stream(2, 3)
     mask = torch.from_numpy(rng.dropout_keep_mask(mix_seed(2, 3, INPUT_SLOT), 300, 7, 0.4)).bool().cuda()
-    dropped = torch.where(mask, x * (1.0 / (1.0 - torch.full((), 0.4, device="cuda"))), torch.zeros((), device="cuda"))
-    # (the kernel's 1 / (1 - p) is formed in fp32 from the fp32 rate, as here)
+    dropped = torch.where(mask, x * torch.full((), 1.0 / (1.0 - 0.4), device="cuda"), torch.zeros((), device="cuda"))
     assert torch.equal(m(x, ei).detach(), plain(dropped, ei).detach())
     m.eval()
     assert torch.equal(m(x, ei).detach(), want)
