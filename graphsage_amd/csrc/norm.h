@@ -34,11 +34,13 @@ struct NormBwd {
 // same whatever they hold, so a row takes the fewest lanes that need no more than three vectors each, which also leaves
 // few of them idle (fp16, 126 MB tables, forward + backward with residual and dropout: 264 columns in 16 lanes x 3 run at
 // 4.6 and 4.0 TB/s, in 64 x 1 at 3.5 and 3.6; 1544 columns as a workgroup of 193 threads x 1 4.0, 97 x 2 4.2).  Two or
-// four waves a row rather than three or five: eight fit a compute unit.  Large tables of whole cache lines without
+// four waves a row rather than three or five: eight fit a compute unit.  Past 8192 columns (NORM_W) 16 elements a thread in
+// up to sixteen waves, as many as a compute unit has room for: 8192 x 16000 bf16 forward 97 us, backward 176, joined 143
+// and 304; as eight waves with 32 elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).  Large tables of whole cache lines without
 // residual or dropout stream best where neighbouring lanes hold neighbouring vectors (`stream`: 10 M x 64 fp32 forward
 // 0.94 ms at 16 lanes x 1, 0.99 at 8 x 2; backward 1.41 and 1.58).
 enum NormKind { NORM_ONE, NORM_R4, NORM_R8, NORM_R8x2, NORM_R8x3, NORM_R16, NORM_R16x2, NORM_R16x3, NORM_R32, NORM_R32x2,
-                NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_B8, NORM_LONG };
+                NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_W, NORM_LONG };
 struct NormForm { NormKind kind; int row; };      // threads of a row
 static inline NormForm norm_form(int64_t F, int V, bool stream) {
   if (F < V) return {NORM_ONE, 8};
@@ -62,8 +64,8 @@ static inline NormForm norm_form(int64_t F, int V, bool stream) {
   if (nv <= 512) return {NORM_B2, 256};
   if (nv <= 768) return {NORM_B3, waves(3)};
   if (nv <= 1024) return {NORM_B2, waves(2)};
-  if (nv <= 2048) return {NORM_B4, waves(4)};
-  if (nv <= 4096 && V == 4) return {NORM_B8, waves(8)};
+  if (nv <= 2048 && V == 4) return {NORM_B4, waves(4)};
+  if (nv <= 16384 / V) return {NORM_W, waves(16 / V)};
   return {NORM_LONG, 1024};
 }
 

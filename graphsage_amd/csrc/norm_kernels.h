@@ -214,16 +214,17 @@ template <typename T> struct Ln {
   NormDrop d;
 };
 
-// A row takes TPR lanes of a wave, or (TPR = 0) a.row threads: up to MAXW whole waves.  A workgroup takes as many rows at
+// A row takes TPR lanes of a wave, or a.row threads: up to 8 (TPR = 0) or 16 (TPR = -1) whole waves.  A workgroup takes as many rows at
 // once as fit.  Thread t of the row holds K vectors of V columns, a row's threads apart.  A vector that would go past the
 // row's end is moved back to end with it; its first `lo` elements (all of them, where the thread has nothing left to do)
 // then belong to vectors before it: both threads form and store the same values, the sums count them once.
 constexpr int MAXW = 8;
+constexpr int ln_waves(int TPR) { return TPR < 0 ? 16 : MAXW; }
 template <int V, int TPR, int K> struct Cols {
   int t, threads, col[K], lo[K];
   bool on[K], full;
   __device__ __forceinline__ Cols(int F, int row) {
-    threads = TPR ? TPR : row;
+    threads = TPR > 0 ? TPR : row;
     t = threadIdx.x % threads;
     full = F == threads * K * V;
 #pragma unroll
@@ -294,11 +295,11 @@ struct Walk { int64_t begin, apart, step; int turns; };
 // LOOP: several turns, the row after in flight; otherwise one turn and as many workgroups as that takes, which start in
 // order (see dropout_k: 1 M x 128 fp32 0.165 ms, 0.178 as a loop over the grid the GPU holds, joined 0.237 and 0.272).
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT, bool LOOP>
-__global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW) ln_fwd_k(Ln<T> a, Walk g, float eps, T *y, T *sum, float *mean, float *rstd) {
-  constexpr bool AHEAD = LOOP && K * V < 32;  // 32 elements a thread: no registers left for the row after
-  __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
+__global__ void __launch_bounds__(TPR > 0 || K == 3 ? 256 : 64 * ln_waves(TPR)) ln_fwd_k(Ln<T> a, Walk g, float eps, T *y, T *sum, float *mean, float *rstd) {
+  constexpr int WAVES = ln_waves(TPR);
+  __shared__ float part[TPR > 0 ? 1 : 2][TPR > 0 ? 1 : WAVES][2];
   const Cols<V, TPR, K> c(a.F, a.row);
-  const int first = TPR ? threadIdx.x / (TPR ? TPR : 1) : 0;      // this thread's among the rows at once
+  const int first = TPR > 0 ? threadIdx.x / (TPR > 0 ? TPR : 1) : 0;      // this thread's among the rows at once
   int64_t row = g.begin + (int64_t)blockIdx.x * g.apart + first;
   Operands<T, V, TPR, K, JOIN, NT> next;
   const auto fetch = [&](int64_t r) { next.load(a, c, r < a.M ? r : a.M - 1); };
@@ -320,16 +321,15 @@ __global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW) ln_fwd_k(Ln<T
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
   // (rows of several waves) this wave's elements, and those of the wave whose sums this lane puts together
-  const int mine = TPR ? 0 : c.wave_count(c.t >> 6, a.F), other = TPR ? 0 : c.wave_count(threadIdx.x % MAXW, a.F);
+  const int mine = TPR > 0 ? 0 : c.wave_count(c.t >> 6, a.F), other = TPR > 0 ? 0 : c.wave_count(threadIdx.x % WAVES, a.F);
   const float inv_mine = mine ? 1.0f / (float)mine : 0.f, inv_other = other ? 1.0f / (float)other : 0.f;
   if (LOOP) weights();
   const int turns = LOOP ? g.turns : 1;
   for (int turn = 0; turn < turns; ++turn, row += g.step) {
     float z[K][V];
     bool kept[K][V];
-    if (!AHEAD && turn > 0) fetch(row);
     next.z(a, c, row, key, thr, z, kept);
-    if (AHEAD && turn + 1 < turns) fetch(row + g.step);
+    if (LOOP && turn + 1 < turns) fetch(row + g.step);
     float s = 0.f, q = 0.f, m, var;
     const auto squares = [&](float about) {
       if (c.full) {
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW) ln_fwd_k(Ln<T
 #pragma unroll
         for (int i = 0; i < V; ++i) s += c.live(k, i) ? z[k][i] : 0.f;
     }
-    if constexpr (TPR != 0) {
+    if constexpr (TPR > 0) {
       m = lanes_sum<TPR>(s) * inv_f;
       squares(m);
       var = lanes_sum<TPR>(q) * inv_f;
@@ -370,10 +370,10 @@ __global__ void __launch_bounds__(TPR || K == 3 ? 256 : 64 * MAXW) ln_fwd_k(Ln<T
       if (gs_lane() == 0) { slot[c.t >> 6][0] = sw; slot[c.t >> 6][1] = q; }
       __syncthreads();
       // (waves that are not there have no elements; their slots hold whatever LDS held)
-      const float so = other ? slot[threadIdx.x % MAXW][0] : 0.f, qo = other ? slot[threadIdx.x % MAXW][1] : 0.f;
-      m = lanes_sum<MAXW>(so) * inv_f;
+      const float so = other ? slot[threadIdx.x % WAVES][0] : 0.f, qo = other ? slot[threadIdx.x % WAVES][1] : 0.f;
+      m = lanes_sum<WAVES>(so) * inv_f;
       const float e = so * inv_other - m;
-      var = lanes_sum<MAXW>(fmaf(e * e, (float)other, qo)) * inv_f;
+      var = lanes_sum<WAVES>(fmaf(e * e, (float)other, qo)) * inv_f;
     }
     const float rs = rsqrtf(var + eps);
     if (!LOOP) weights();
@@ -408,11 +408,13 @@ constexpr int FLUSH = 16;
 
 // Workgroups of eight waves (fewer slabs than four would leave).  With 24 elements a thread and the row after in flight
 // four have the registers: rows of several waves do better so (bf16 6000 columns joined backward 205 us, without the row
-// after 215), rows within a wave with eight waves and no row ahead (fp16 257 columns 79 -> 74 us, 1200 137 -> 128).
+// after 215), rows within a wave with eight waves and no row ahead (fp16 257 columns 79 -> 74 us, 1200 137 -> 128).  Of
+// sixteen waves each has 128 registers: no row ahead, and grad_sum is read only when the weights are used up (fp32 8192 x
+// 16000 joined 661 us; with the other operands 758).
 constexpr bool ln_bwd_ahead(int V, int TPR, int K, bool JOIN) {
-  return K * V < (TPR ? 24 : 32) && !(JOIN && K * V == 16 && V == 4);
+  return TPR >= 0 && (TPR == 0 || K * V < 24) && !(JOIN && K * V == 16 && V == 4);
 }
-constexpr int ln_bwd_threads(int V, int TPR, int K) { return K == 3 && V == 8 && TPR == 0 ? 256 : 64 * MAXW; }
+constexpr int ln_bwd_threads(int V, int TPR, int K) { return K == 3 && V == 8 && TPR == 0 ? 256 : 64 * ln_waves(TPR); }
 
 // Nothing of this wave is under way (vmcnt = 0).  The loops over the grid that the GPU holds wait so before their stores and
 // after them on streamed tables: reads and writes then come in turns, which the memory takes better than both at once
@@ -424,11 +426,12 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
   constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
   constexpr int A = AHEAD ? K : 1;
   extern __shared__ float acc[];              // [2 K V][threads]: grad_w, then grad_b; a thread's words are its own
-  __shared__ float part[TPR ? 1 : 2][TPR ? 1 : MAXW][2];
+  constexpr int WAVES = ln_waves(TPR);
+  __shared__ float part[TPR > 0 ? 1 : 2][TPR > 0 ? 1 : WAVES][2];
   constexpr int threads = ln_bwd_threads(V, TPR, K);      // (a workgroup a row may have fewer)
   float *const mine = acc + threadIdx.x;
   const Cols<V, TPR, K> c(a.F, a.row);
-  const int rows = TPR ? threads / (TPR ? TPR : 1) : blockDim.x / c.threads, first = threadIdx.x / c.threads;
+  const int rows = TPR > 0 ? threads / (TPR > 0 ? TPR : 1) : blockDim.x / c.threads, first = TPR < 0 ? 0 : threadIdx.x / c.threads;
   int64_t base = g.begin + (int64_t)blockIdx.x * g.apart, row = base + first;
   Operands<T, V, TPR, K, JOIN, NT> next;
   Raw<T, V> gnext[K], snext[JOIN ? K : 1];
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
     next.load(a, c, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) gnext[k].template load<NT>(d.g + r * a.F + c.col[k]);
-    if (JOIN && d.gsum)
+    if (JOIN && d.gsum && TPR >= 0)
 #pragma unroll
       for (int k = 0; k < K; ++k) snext[k].template load<NT>(d.gsum + r * a.F + c.col[k]);
     mnext = d.mean[r];
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       gnext[k].open(gv[k]);
-      if (JOIN) sv[k] = snext[k];
+      if (JOIN && TPR >= 0) sv[k] = snext[k];
     }
     const float m = mnext, rs = rnext;
     if (AHEAD && turn + 1 < g.turns) fetch(row + g.step);
@@ -505,6 +508,9 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
         }
         gv[k][i] *= w[k][i];
       }
+    if (JOIN && TPR < 0 && d.gsum)
+#pragma unroll
+      for (int k = 0; k < K; ++k) sv[k].template load<NT>(d.gsum + (row < a.M ? row : a.M - 1) * a.F + c.col[k]);
     if (a.F % V == 0) {                     // (g is zero where a thread has no column)
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -516,7 +522,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
 #pragma unroll
         for (int i = 0; i < V; ++i) { const float e = c.live(k, i) ? gv[k][i] : 0.f; s1 += e; s2 = fmaf(e, h[k][i], s2); }
     }
-    if constexpr (TPR != 0) {
+    if constexpr (TPR > 0) {
       s1 = lanes_sum<TPR>(s1);
       s2 = lanes_sum<TPR>(s2);
     } else {
@@ -525,9 +531,9 @@ __global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, W
       float(*slot)[2] = part[turn & 1] + first * (c.threads >> 6);
       if (gs_lane() == 0) { slot[c.t >> 6][0] = s1; slot[c.t >> 6][1] = s2; }
       __syncthreads();
-      const bool there = threadIdx.x % MAXW < c.threads >> 6;
-      s1 = lanes_sum<MAXW>(there ? slot[threadIdx.x % MAXW][0] : 0.f);
-      s2 = lanes_sum<MAXW>(there ? slot[threadIdx.x % MAXW][1] : 0.f);
+      const bool there = threadIdx.x % WAVES < c.threads >> 6;
+      s1 = lanes_sum<WAVES>(there ? slot[threadIdx.x % WAVES][0] : 0.f);
+      s2 = lanes_sum<WAVES>(there ? slot[threadIdx.x % WAVES][1] : 0.f);
     }
     s1 *= inv_f;
     s2 *= inv_f;
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(1024) ln_slabs_k(const float *ws, int slabs, i
   }
 }
 
-// ------------------------------------------------------------------ rows longer than a workgroup's registers
+// ------------------------------------------------------------------ rows longer than a workgroup's registers (16 384)
 __device__ __forceinline__ float block_sum(float v) {      // over 1024 threads, in every thread
   __shared__ float part[16];
   v = lanes_sum<64>(v);
@@ -625,66 +631,124 @@ __device__ __forceinline__ float block_sum(float v) {      // over 1024 threads,
   return v;
 }
 
-template <typename T> __device__ __forceinline__ float weight1(const void *w, int wdtype, int c, float other) {
-  Weights<T, 1> r;
-  float f[1];
-  r.load(w, wdtype, c);
-  r.open(w, wdtype, other, f);
-  return f[0];
-}
+// Thread t's vectors of a row are t, t + 1024, ... ; the last of the row is moved back as in Cols
+template <typename T> struct LongVec {
+  static constexpr int V = Tab<T>::V;
+  int c, lo;
+  __device__ __forceinline__ LongVec(int v, int F) : c(v < F - V ? v : F - V) { lo = v - c; }
+  __device__ __forceinline__ void z(const Ln<T> &a, int64_t base, uint64_t key, uint32_t thr, float (&z)[V], bool (&kept)[V]) const {
+    Raw<T, V> x, r;
+    x.load(a.x + base + c);
+    if (a.res) r.load(a.res + base + c);
+    x.open(z);
+    if (a.d.p > 0.f) {
+      draw_vec<V>(kept, (uint64_t)(base + c), key, thr, a.d.p);
+      drop_vec<V>(z, kept, a.d.inv_keep);
+    }
+    if (!a.res) return;
+    float q[V];
+    r.open(q);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] += q[i];
+  }
+  __device__ __forceinline__ void weight(const void *w, int wdtype, float other, float (&f)[V]) const {
+    Weights<T, V> r;
+    r.load(w, wdtype, c);
+    r.open(w, wdtype, other, f);
+  }
+};
 
-template <typename T> __device__ __forceinline__ float long_z(const Ln<T> &a, int64_t idx, uint64_t key) {
-  float v = (float)a.x[idx];
-  if (a.d.p > 0.f) v = dropout_keep(key, (uint64_t)idx, a.d.p) ? v * a.d.inv_keep : 0.f;
-  return a.res ? (float)a.res[idx] + v : v;
-}
-
+// A row is read twice (from the caches where it has stayed there): for its mean and squares about it, which a thread takes
+// along from vector to vector (each vector about its own mean, then the two put together), and for y.  Bound by the second
+// read and by a thread's few loads in flight: 4096 x 32768 fp32 0.28 ms, joined 0.38, backward 0.66 and 0.99 (bf16 0.17,
+// 0.27, 0.36, 0.57).
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_fwd_long_k(Ln<T> a, float eps, T *y, T *sum, float *mean, float *rstd) {
+  constexpr int V = Tab<T>::V;
   const uint64_t key = drop_key(a.d);
+  const uint32_t thr = dropout_threshold(a.d.p);
   const float inv_f = 1.0f / (float)a.F;
   for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
     const int64_t base = r * a.F;
-    float s = 0.f, q = 0.f;
-    for (int c = threadIdx.x; c < a.F; c += 1024) s += long_z(a, base + c, key);
-    const float m = block_sum(s) * inv_f;
-    for (int c = threadIdx.x; c < a.F; c += 1024) { const float e = long_z(a, base + c, key) - m; q = fmaf(e, e, q); }
-    const float rs = 1.0f / sqrtf(block_sum(q) * inv_f + eps);
-    for (int c = threadIdx.x; c < a.F; c += 1024) {
-      const float z = long_z(a, base + c, key);
-      const float w = weight1<T>(a.w, a.wdtype, c, 1.f), b = weight1<T>(a.b, a.wdtype, c, 0.f);
-      y[base + c] = (T)fmaf((z - m) * rs, w, b);
-      if (sum) sum[base + c] = (T)z;
+    float n = 0.f, m = 0.f, q = 0.f, z[V];
+    bool kept[V];
+    for (int v = threadIdx.x * V; v < a.F; v += 1024 * V) {
+      const LongVec<T> at(v, a.F);
+      at.z(a, base, key, thr, z, kept);
+      float s = 0.f, qv = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += i >= at.lo ? z[i] : 0.f;
+      const float nv = (float)(V - at.lo), mv = s / nv;
+#pragma unroll
+      for (int i = 0; i < V; ++i) { const float e = i >= at.lo ? z[i] - mv : 0.f; qv = fmaf(e, e, qv); }
+      const float all = n + nv, e = mv - m;
+      m = fmaf(e, nv / all, m);
+      q += fmaf(e * e, n * nv / all, qv);
+      n = all;
     }
-    if (mean && threadIdx.x == 0) { mean[r] = m; rstd[r] = rs; }
+    const float mr = block_sum(m * n) * inv_f, e = m - mr;
+    const float rs = 1.0f / sqrtf(block_sum(fmaf(e * e, n, q)) * inv_f + eps);
+    for (int v = threadIdx.x * V; v < a.F; v += 1024 * V) {
+      const LongVec<T> at(v, a.F);
+      float w[V], b[V];
+      at.z(a, base, key, thr, z, kept);
+      at.weight(a.w, a.wdtype, 1.f, w);
+      at.weight(a.b, a.wdtype, 0.f, b);
+      if (sum) Raw<T, V>::store(sum + base + at.c, z);
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = fmaf((z[i] - mr) * rs, w[i], b[i]);
+      Raw<T, V>::store(y + base + at.c, z);
+    }
+    if (mean && threadIdx.x == 0) { mean[r] = mr; rstd[r] = rs; }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const T *gsum, const float *mean,
                                                      const float *rstd, T *gx, T *gres) {
+  constexpr int V = Tab<T>::V;
   const uint64_t key = drop_key(a.d);
+  const uint32_t thr = dropout_threshold(a.d.p);
   const float inv_f = 1.0f / (float)a.F;
   for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
     const int64_t base = r * a.F;
     const float m = mean[r], rs = rstd[r];
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = threadIdx.x; c < a.F; c += 1024) {
-      const float h = (long_z(a, base + c, key) - m) * rs;
-      const float e = (float)g[base + c] * weight1<T>(a.w, a.wdtype, c, 1.f);
-      s1 += e;
-      s2 = fmaf(e, h, s2);
+    float s1 = 0.f, s2 = 0.f, h[V], e[V], w[V];
+    bool kept[V];
+    const auto row = [&](const LongVec<T> &at) {      // h and g w of these columns
+      Raw<T, V> gr;
+      gr.load(g + base + at.c);
+      at.z(a, base, key, thr, h, kept);
+      at.weight(a.w, a.wdtype, 1.f, w);
+      gr.open(e);
+#pragma unroll
+      for (int i = 0; i < V; ++i) { h[i] = (h[i] - m) * rs; e[i] *= w[i]; }
+    };
+    for (int v = threadIdx.x * V; v < a.F; v += 1024 * V) {
+      const LongVec<T> at(v, a.F);
+      row(at);
+#pragma unroll
+      for (int i = 0; i < V; ++i) { const float one = i >= at.lo ? e[i] : 0.f; s1 += one; s2 = fmaf(one, h[i], s2); }
     }
     s1 = block_sum(s1) * inv_f;
     s2 = block_sum(s2) * inv_f;
-    for (int c = threadIdx.x; c < a.F; c += 1024) {
-      const int64_t i = base + c;
-      const float h = (long_z(a, i, key) - m) * rs;
-      const float e = (float)g[i] * weight1<T>(a.w, a.wdtype, c, 1.f);
-      float dz = rs * (e - s1 - h * s2);
-      if (gsum) dz += (float)gsum[i];
-      if (gres) gres[i] = (T)dz;
-      if (gx) gx[i] = (T)(a.d.p <= 0.f ? dz : dropout_keep(key, (uint64_t)i, a.d.p) ? dz * a.d.inv_keep : 0.f);
+    for (int v = threadIdx.x * V; v < a.F; v += 1024 * V) {
+      const LongVec<T> at(v, a.F);
+      row(at);
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = rs * fmaf(-h[i], s2, e[i] - s1);
+      if (gsum) {
+        Raw<T, V> sr;
+        float q[V];
+        sr.load(gsum + base + at.c);
+        sr.open(q);
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] += q[i];
+      }
+      if (gres) Raw<T, V>::store(gres + base + at.c, e);
+      if (!gx) continue;
+      if (a.d.p > 0.f) drop_vec<V>(e, kept, a.d.inv_keep);
+      Raw<T, V>::store(gx + base + at.c, e);
     }
   }
 }
@@ -696,20 +760,36 @@ __device__ __forceinline__ void add_carry(float &acc, float &carry, float v) {
   acc = t;
 }
 
+// A vector of columns a thread, rows blockIdx.y, blockIdx.y + gridDim.y, ... -> slab blockIdx.y
 template <typename T>
 __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const float *mean, const float *rstd, float *ws) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.F) return;
+  constexpr int V = Tab<T>::V;
+  const int v = (blockIdx.x * 256 + threadIdx.x) * V;
+  if (v >= a.F) return;
+  const LongVec<T> at(v, a.F);
   const uint64_t key = drop_key(a.d);
-  float dw = 0.f, db = 0.f, dwc = 0.f, dbc = 0.f;
+  const uint32_t thr = dropout_threshold(a.d.p);
+  float dw[V] = {}, db[V] = {}, dwc[V] = {}, dbc[V] = {}, h[V], e[V];
+  bool kept[V];
   for (int64_t r = blockIdx.y; r < a.M; r += gridDim.y) {
-    const float gv = (float)g[r * a.F + c];
-    add_carry(dw, dwc, gv * ((long_z(a, r * a.F + c, key) - mean[r]) * rstd[r]));
-    add_carry(db, dbc, gv);
+    Raw<T, V> gr;
+    gr.load(g + r * a.F + at.c);
+    at.z(a, r * a.F, key, thr, h, kept);
+    gr.open(e);
+    const float m = mean[r], rs = rstd[r];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      add_carry(dw[i], dwc[i], e[i] * ((h[i] - m) * rs));
+      add_carry(db[i], dbc[i], e[i]);
+    }
   }
   float *slab = ws + (int64_t)blockIdx.y * 2 * a.F;
-  slab[c] = dw;
-  slab[a.F + c] = db;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (i < at.lo) continue;
+    slab[at.c + i] = dw[i];
+    slab[a.F + at.c + i] = db[i];
+  }
 }
 
 // ------------------------------------------------------------------ launches
@@ -717,7 +797,7 @@ constexpr int64_t MAX_GRID = 1 << 20;      // workgroups of a launch (a launch's
 
 // Workgroups of this kernel that the GPU holds at once: the rows are dealt out to these, none waits for a place
 template <auto KERNEL> int ln_resident(int threads, int lds) {
-  static std::atomic<int> known[MAXW + 1];
+  static std::atomic<int> known[16 + 1];
   std::atomic<int> &n = known[threads / 64];
   int blocks = n.load(std::memory_order_relaxed);
   if (blocks == 0) {
@@ -731,7 +811,7 @@ template <auto KERNEL> int ln_resident(int threads, int lds) {
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT, bool LOOP>
 void ln_fwd_launch(const Ln<T> &a, int turns, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
   constexpr auto kernel = ln_fwd_k<T, V, TPR, K, JOIN, NT, LOOP>;
-  const int threads = TPR ? 256 : a.row, rows = threads / a.row;
+  const int threads = TPR > 0 ? 256 : a.row, rows = threads / a.row;
   if (turns > 0) {      // neighbouring rows, workgroups in order
     const int64_t apart = (int64_t)rows * turns;
     for (int64_t begin = 0; begin < a.M; begin += MAX_GRID * apart) {
@@ -750,13 +830,13 @@ void ln_fwd_launch(const Ln<T> &a, int turns, float eps, T *y, T *sum, float *me
 // One turn a workgroup, where it has 3200 bytes of rows to spread its weights over (fp32 2 M x 28: 81 us, 83 as a loop of
 // two turns; 2 M x 20: 70 us, as a loop 60; 4 M x 4 59 and 41); 16-bit rows without dropout or a residual need two (less
 // arithmetic a byte: 4 M x 64 bf16 0.165 against 0.191 ms), and so do rows of two or four waves.  Rows of
-// three waves and of 32 elements a thread run as loops over the grid that the GPU holds (8191 x 5120 bf16 33 us, 36 in
-// order; 8192 x 16000 100 us, 108).
+// several waves with three vectors a thread or more, and of more than eight waves, run as loops over the grid that the GPU
+// holds (8191 x 5120 bf16 33 us, 36 in order).
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
-  const int64_t bytes = 256 / (TPR ? TPR : 256) * (int64_t)a.F * sizeof(T);
+  const int64_t bytes = 256 / (TPR > 0 ? TPR : 256) * (int64_t)a.F * sizeof(T);
   constexpr bool thin = sizeof(T) == 2 && !JOIN;
-  if constexpr (TPR == 0) ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, K == 2 ? 2 : 0, eps, y, sum, mean, rstd, st);
+  if constexpr (TPR <= 0) ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, K == 2 && TPR == 0 ? 2 : 0, eps, y, sum, mean, rstd, st);
   else if constexpr (thin || K == 1) {
     if (thin || bytes < 3200)
       ln_fwd_launch<T, V, TPR, K, JOIN, NT, true>(a, bytes < 4096 ? (int)((8191 + bytes) / bytes) : 2, eps, y, sum, mean, rstd, st);
@@ -767,7 +847,7 @@ void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd
 // -> the slabs of column sums that are left in ws
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
-  constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT && K * V < 32>;      // (32 elements: its waits cost registers it has not)
+  constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT>;
   constexpr int lds = 2 * K * V * ln_bwd_threads(V, TPR, K) * (int)sizeof(float);
   const int rows = ln_bwd_threads(V, TPR, K) / a.row, threads = rows * a.row, resident = ln_resident<kernel>(threads, lds);
   // Streamed fp32 tables of short rows in order, as the forward takes them, two turns a workgroup and a slab for each:
@@ -796,7 +876,8 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   CASE(NORM_ONE, 1, 8, 1) CASE(NORM_R4, V, 4, 1) CASE(NORM_R8, V, 8, 1) CASE(NORM_R8x2, V, 8, 2)              \
   CASE(NORM_R8x3, V, 8, 3) LINE(NORM_R16, V, 16, 1) CASE(NORM_R16x2, V, 16, 2) CASE(NORM_R16x3, V, 16, 3)     \
   LINE(NORM_R32, V, 32, 1) CASE(NORM_R32x2, V, 32, 2) CASE(NORM_R32x3, V, 32, 3) LINE(NORM_R64, V, 64, 1)     \
-  CASE(NORM_R64x2, V, 64, 2) CASE(NORM_R64x3, V, 64, 3) CASE(NORM_B2, V, 0, 2) CASE(NORM_B3, V, 0, 3) CASE(NORM_B4, V, 0, 4)
+  CASE(NORM_R64x2, V, 64, 2) CASE(NORM_R64x3, V, 64, 3) CASE(NORM_B2, V, 0, 2) CASE(NORM_B3, V, 0, 3)                          \
+  CASE(NORM_W, V, -1, 16 / V)
 
 template <typename T>
 int ln_fwd(const NormFwd &n, hipStream_t st) {
@@ -815,10 +896,10 @@ int ln_fwd(const NormFwd &n, hipStream_t st) {
   case KIND: ln_fwd_go<T, V, TPR, K, false, true>(ARGS); break;
   switch (f.kind) {
     LN_FORMS(CASE, LINE)
-    case NORM_B8:
+    case NORM_B4:      // (16-bit rows as long take NORM_W)
       if constexpr (V == 4) {
-        if (join) ln_fwd_go<T, V, 0, 8, true, false>(ARGS);
-        else ln_fwd_go<T, V, 0, 8, false, false>(ARGS);
+        if (join) { if (nt) ln_fwd_go<T, V, 0, 4, true, true>(ARGS); else ln_fwd_go<T, V, 0, 4, true, false>(ARGS); }
+        else { if (nt) ln_fwd_go<T, V, 0, 4, false, true>(ARGS); else ln_fwd_go<T, V, 0, 4, false, false>(ARGS); }
       }
       break;
     case NORM_LONG:
@@ -850,16 +931,17 @@ int ln_bwd(const NormBwd &n, hipStream_t st) {
   case KIND: slabs = ln_bwd_go<T, V, TPR, K, false, true>(a, d, st); break;
     switch (f.kind) {
       LN_FORMS(CASE, LINE)
-      case NORM_B8:
+      case NORM_B4:
         if constexpr (V == 4)
-          slabs = join ? ln_bwd_go<T, V, 0, 8, true, false>(a, d, st) : ln_bwd_go<T, V, 0, 8, false, false>(a, d, st);
+          slabs = join ? (nt ? ln_bwd_go<T, V, 0, 4, true, true>(a, d, st) : ln_bwd_go<T, V, 0, 4, true, false>(a, d, st))
+                       : (nt ? ln_bwd_go<T, V, 0, 4, false, true>(a, d, st) : ln_bwd_go<T, V, 0, 4, false, false>(a, d, st));
         break;
       case NORM_LONG:
         if (d.gx || d.gres)
           hipLaunchKernelGGL(ln_dz_long_k<T>, dim3(gs_grid(n.M, 1, 512)), dim3(1024), 0, st, a, d.g, d.gsum, d.mean, d.rstd,
                              d.gx, d.gres);
         if (d.ws)
-          hipLaunchKernelGGL(ln_dw_long_k<T>, dim3((unsigned)((n.F + 255) / 256), slabs), dim3(256), 0, st, a, d.g, d.mean,
+          hipLaunchKernelGGL(ln_dw_long_k<T>, dim3((unsigned)((n.F + 256 * V - 1) / (256 * V)), slabs), dim3(256), 0, st, a, d.g, d.mean,
                              d.rstd, d.ws);
     }
 #undef CASE
