@@ -32,17 +32,18 @@ struct NormBwd {
 // Which kernel a row takes: K vectors of 16 bytes (V elements each) in each of R lanes of a wave, or of `row` threads of a
 // workgroup (B); NORM_ONE: rows shorter than a vector, an element a lane.  A row's sums and addresses cost its threads the
 // same whatever they hold, so a row takes the fewest lanes that need no more than three vectors each, which also leaves
-// few of them idle (fp16, 126 MB tables, forward + backward with residual and dropout: 264 columns in 16 lanes x 3 run at
-// 4.6 and 4.0 TB/s, in 64 x 1 at 3.5 and 3.6; 1544 columns as a workgroup of 193 threads x 1 4.0, 97 x 2 4.2).  Two or
+// few of them idle (fp16 240 000 x 264, joined: 16 lanes x 3 78 us forward and 135 backward, 32 x 2 92 and 167).  Two or
 // four waves a row rather than three or five: eight fit a compute unit.  Past 8192 columns (NORM_W) 16 elements a thread in
 // up to sixteen waves, as many as a compute unit has room for: 8192 x 16000 bf16 forward 97 us, backward 176, joined 143
-// and 304; as eight waves with 32 elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).  Large tables of whole cache lines without
-// residual or dropout stream best where neighbouring lanes hold neighbouring vectors (`stream`: 10 M x 64 fp32 forward
-// 0.94 ms at 16 lanes x 1, 0.99 at 8 x 2; backward 1.41 and 1.58).
+// and 304; as eight waves with 32 elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).
+// Large fp32 tables of whole cache lines without residual or dropout stream best where neighbouring lanes hold
+// neighbouring vectors (`stream`: 10 M x 64 forward 0.81 ms at 16 lanes x 1, 0.85 at 8 x 2, backward 1.25 and 1.34; 4 M x
+// 128 0.65 and 0.68, 1.01 and 1.08; bf16 2 M x 256 0.325 and 0.319, 0.548 and 0.541).
 enum NormKind { NORM_ONE, NORM_R4, NORM_R8, NORM_R8x2, NORM_R8x3, NORM_R16, NORM_R16x2, NORM_R16x3, NORM_R32, NORM_R32x2,
                 NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_W, NORM_LONG };
 struct NormForm { NormKind kind; int row; };      // threads of a row
 static inline NormForm norm_form(int64_t F, int V, bool stream) {
+  stream = stream && V == 4;
   if (F < V) return {NORM_ONE, 8};
   const int64_t nv = (F + V - 1) / V;
   const auto waves = [&](int k) { return (int)((nv + 64 * k - 1) / (64 * k)) * 64; };
@@ -75,8 +76,9 @@ static inline int norm_blocks(int64_t M, int rows, int cap) {
   return groups ? (int)((groups + turns - 1) / turns) : 0;
 }
 // Tables too large for any cache (256 MB behind the L2s) are read and written past them, if their rows share no cache
-// lines: 10 M x 64 fp32 forward 1.09 -> 1.03 ms, joined 1.86 -> 1.68; a 15 MB table loses that way (7.1 -> 11.8 us), for
-// the caches serve it, and so does 1 M x 196 fp16 (joined forward 4.7 -> 4.1 TB/s).
+// lines: 1 M x 128 fp32 joined forward 0.263 -> 0.242 ms, backward 0.454 -> 0.414; 10 M x 64 backward 1.43 -> 1.25.
+// Smaller ones lose that way, for the caches serve them (60 000 x 64 joined forward 9.1 -> 9.8 us), and so do rows that end
+// inside a line (1 M x 196 fp16 forward 0.141 -> 0.156 ms, joined backward 0.388 -> 0.476).
 static inline bool norm_large(int64_t n, size_t size) { return n * (int64_t)size >= ((int64_t)256 << 20); }
 static inline bool norm_streams(int64_t M, int64_t F, size_t size) { return norm_large(M * F, size) && F * (int64_t)size % 128 == 0; }
 

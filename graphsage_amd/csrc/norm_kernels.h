@@ -293,7 +293,8 @@ struct Walk { int64_t begin, apart, step; int turns; };
 
 // ------------------------------------------------------------------ forward
 // LOOP: several turns, the row after in flight; otherwise one turn and as many workgroups as that takes, which start in
-// order (see dropout_k: 1 M x 128 fp32 0.165 ms, 0.178 as a loop over the grid the GPU holds, joined 0.237 and 0.272).
+// order (see dropout_k: 1 M x 128 fp32 0.163 ms, 0.178 as a loop over the grid the GPU holds, joined 0.242 and 0.272: the
+// memory's rate for such a stream, 6.3 TB/s).
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT, bool LOOP>
 __global__ void __launch_bounds__(TPR > 0 || K == 3 ? 256 : 64 * ln_waves(TPR)) ln_fwd_k(Ln<T> a, Walk g, float eps, T *y, T *sum, float *mean, float *rstd) {
   constexpr int WAVES = ln_waves(TPR);
@@ -406,29 +407,29 @@ template <typename T> struct Grads {
 // for the first level either every row goes to LDS.
 constexpr int FLUSH = 16;
 
-// Workgroups of eight waves (fewer slabs than four would leave).  With 24 elements a thread and the row after in flight
-// four have the registers: rows of several waves do better so (bf16 6000 columns joined backward 205 us, without the row
-// after 215), rows within a wave with eight waves and no row ahead (fp16 257 columns 79 -> 74 us, 1200 137 -> 128).  Of
-// sixteen waves each has 128 registers: no row ahead, and grad_sum is read only when the weights are used up (fp32 8192 x
-// 16000 joined 661 us; with the other operands 758).
+// Workgroups of eight waves (fewer slabs than four would leave), or of the row's up to sixteen.  The row after is loaded a
+// row ahead where there are registers for it: not at 24 elements a thread (fp16 257 columns 39 us, joined 71; with four
+// waves that have them 42 and 83; 6000 columns joined 212 and 217), nor at 16 of fp32 joined, nor of sixteen waves, which
+// have 128 each; those read grad_sum, too, only when the weights are used up (fp32 8192 x 16000 joined 661 us; with the
+// other operands 758).
 constexpr bool ln_bwd_ahead(int V, int TPR, int K, bool JOIN) {
-  return TPR >= 0 && (TPR == 0 || K * V < 24) && !(JOIN && K * V == 16 && V == 4);
+  return TPR >= 0 && K * V < 24 && !(JOIN && K * V == 16 && V == 4);
 }
-constexpr int ln_bwd_threads(int V, int TPR, int K) { return K == 3 && V == 8 && TPR == 0 ? 256 : 64 * ln_waves(TPR); }
+constexpr int ln_bwd_threads(int TPR) { return 64 * ln_waves(TPR); }
 
 // Nothing of this wave is under way (vmcnt = 0).  The loops over the grid that the GPU holds wait so before their stores and
 // after them on streamed tables: reads and writes then come in turns, which the memory takes better than both at once
-// (10 M x 64 fp32 joined backward 2.36 against 2.50 ms, 1 M x 256 0.87 against 0.97).
+// (1 M x 256 fp32 backward 0.52 ms against 0.54, joined 0.90 against 0.98; 1 M x 128 joined 0.414 against 0.434).
 __device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
-__global__ void __launch_bounds__(ln_bwd_threads(V, TPR, K)) ln_bwd_k(Ln<T> a, Walk g, Grads<T> d) {
+__global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g, Grads<T> d) {
   constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
   constexpr int A = AHEAD ? K : 1;
   extern __shared__ float acc[];              // [2 K V][threads]: grad_w, then grad_b; a thread's words are its own
   constexpr int WAVES = ln_waves(TPR);
   __shared__ float part[TPR > 0 ? 1 : 2][TPR > 0 ? 1 : WAVES][2];
-  constexpr int threads = ln_bwd_threads(V, TPR, K);      // (a workgroup a row may have fewer)
+  constexpr int threads = ln_bwd_threads(TPR);      // (a workgroup a row may have fewer)
   float *const mine = acc + threadIdx.x;
   const Cols<V, TPR, K> c(a.F, a.row);
   const int rows = TPR > 0 ? threads / (TPR > 0 ? TPR : 1) : blockDim.x / c.threads, first = TPR < 0 ? 0 : threadIdx.x / c.threads;
@@ -829,9 +830,9 @@ void ln_fwd_launch(const Ln<T> &a, int turns, float eps, T *y, T *sum, float *me
 
 // One turn a workgroup, where it has 3200 bytes of rows to spread its weights over (fp32 2 M x 28: 81 us, 83 as a loop of
 // two turns; 2 M x 20: 70 us, as a loop 60; 4 M x 4 59 and 41); 16-bit rows without dropout or a residual need two (less
-// arithmetic a byte: 4 M x 64 bf16 0.165 against 0.191 ms), and so do rows of two or four waves.  Rows of
+// arithmetic a byte: 4 M x 64 bf16 0.167 against 0.181 ms), and so do rows of two or four waves.  Rows of
 // several waves with three vectors a thread or more, and of more than eight waves, run as loops over the grid that the GPU
-// holds (8191 x 5120 bf16 33 us, 36 in order).
+// holds (8191 x 5120 bf16 33 us, 42 in order).
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
   const int64_t bytes = 256 / (TPR > 0 ? TPR : 256) * (int64_t)a.F * sizeof(T);
@@ -848,11 +849,11 @@ void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT>;
-  constexpr int lds = 2 * K * V * ln_bwd_threads(V, TPR, K) * (int)sizeof(float);
-  const int rows = ln_bwd_threads(V, TPR, K) / a.row, threads = rows * a.row, resident = ln_resident<kernel>(threads, lds);
+  constexpr int lds = 2 * K * V * ln_bwd_threads(TPR) * (int)sizeof(float);
+  const int rows = ln_bwd_threads(TPR) / a.row, threads = rows * a.row, resident = ln_resident<kernel>(threads, lds);
   // Streamed fp32 tables of short rows in order, as the forward takes them, two turns a workgroup and a slab for each:
-  // 10 M x 64 1.41 -> 1.22 ms (joined, and in 16 bits, nothing is gained: more arithmetic a byte).  From 32 rows a slab on
-  // the slabs are 2 % of the traffic.
+  // 10 M x 64 1.37 -> 1.25 ms, 4 M x 128 1.06 -> 1.01 (joined, and in 16 bits, nothing is gained: more arithmetic a byte).
+  // From 32 rows a slab on the slabs are 2 % of the traffic.
   constexpr int turns = 2;
   if (NT && !JOIN && d.ws && norm_folds(a.M, a.F, sizeof(T)) && rows * turns >= NORM_FOLD_ROWS) {
     const int blocks = (int)((a.M + rows * turns - 1) / (rows * turns)), folded = norm_blocks(blocks, 1, 256);
@@ -863,7 +864,7 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
     hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * a.F + 15) / 16)), dim3(1024), 0, st, out, folded, a.F, a.wdtype, d.gw, d.gb);
     return 0;
   }
-  // (of the large tables sixteen waves a compute unit keep the memory busy; 24 of them were slower: 1.49 against 1.41 ms)
+  // (of the large tables sixteen waves a compute unit keep the memory busy; 24 of them were slower: 1 M x 256 fp32 0.56 against 0.52 ms)
   const int most = norm_max_slabs(a.M, a.F), held = NT && resident > 512 ? 512 : resident;
   const int slabs = norm_blocks(a.M, rows, held < most ? held : most);
   const int64_t step = (int64_t)slabs * rows;
@@ -871,7 +872,7 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   return slabs > 1 ? slabs : 0;
 }
 
-// every form: CASE(kind, V, TPR, K); LINE: those of large plain tables only
+// every form: CASE(kind, V, TPR, K); LINE: those of large plain fp32 tables only
 #define LN_FORMS(CASE, LINE)                                                                                  \
   CASE(NORM_ONE, 1, 8, 1) CASE(NORM_R4, V, 4, 1) CASE(NORM_R8, V, 8, 1) CASE(NORM_R8x2, V, 8, 2)              \
   CASE(NORM_R8x3, V, 8, 3) LINE(NORM_R16, V, 16, 1) CASE(NORM_R16x2, V, 16, 2) CASE(NORM_R16x3, V, 16, 3)     \
@@ -893,7 +894,7 @@ int ln_fwd(const NormFwd &n, hipStream_t st) {
     else { if (nt) ln_fwd_go<T, V, TPR, K, false, true>(ARGS); else ln_fwd_go<T, V, TPR, K, false, false>(ARGS); }    \
     break;
 #define LINE(KIND, V, TPR, K) \
-  case KIND: ln_fwd_go<T, V, TPR, K, false, true>(ARGS); break;
+  case KIND: if constexpr (V == 4) ln_fwd_go<T, V, TPR, K, false, true>(ARGS); break;
   switch (f.kind) {
     LN_FORMS(CASE, LINE)
     case NORM_B4:      // (16-bit rows as long take NORM_W)
@@ -928,7 +929,7 @@ int ln_bwd(const NormBwd &n, hipStream_t st) {
                  : (nt ? ln_bwd_go<T, V, TPR, K, false, true>(a, d, st) : ln_bwd_go<T, V, TPR, K, false, false>(a, d, st)); \
     break;
 #define LINE(KIND, V, TPR, K) \
-  case KIND: slabs = ln_bwd_go<T, V, TPR, K, false, true>(a, d, st); break;
+  case KIND: if constexpr (V == 4) slabs = ln_bwd_go<T, V, TPR, K, false, true>(a, d, st); break;
     switch (f.kind) {
       LN_FORMS(CASE, LINE)
       case NORM_B4:
