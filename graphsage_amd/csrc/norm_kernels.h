@@ -799,10 +799,17 @@ constexpr int64_t MAX_GRID = 1 << 20;      // workgroups of a launch (a launch's
 // Workgroups of this kernel that the GPU holds at once: the rows are dealt out to these, none waits for a place
 template <auto KERNEL> int ln_resident(int threads, int lds) {
   static std::atomic<int> known[16 + 1];
+  if (lds > 65536) {      // (the attribute is a device's own)
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+      (void)hipFuncSetAttribute((const void *)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+    }
+  }
   std::atomic<int> &n = known[threads / 64];
   int blocks = n.load(std::memory_order_relaxed);
   if (blocks == 0) {
-    if (lds > 65536) (void)hipFuncSetAttribute((const void *)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, KERNEL, threads, lds) != hipSuccess || blocks < 1) blocks = 1;
     n.store(blocks, std::memory_order_relaxed);
   }

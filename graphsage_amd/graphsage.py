@@ -114,6 +114,11 @@ class SAGEConv(nn.Module):
 class GraphSAGE(nn.Module):
     """GraphSAGE encoder (reference ``GraphSAGE``, ``src/model/graphsage.py:33-157``)."""
 
+    # (of models pickled whole before these existed)
+    norm: Optional[str] = None
+    residual = False
+    input_dropout = 0.0
+
     def __init__(self, in_channels: int = 7, hidden_channels: int = 64, out_channels: int = 64,
                  num_layers: int = 2, dropout: float = 0.3, aggregator: str = "mean",
                  normalize_output: bool = True, cache_input_aggregation: bool = False,

@@ -431,7 +431,9 @@ def test_joined_past_2_to_the_32_elements():
     (524_301, 128, torch.float32, True), (262_151, 256, torch.float32, False), (2_100_001, 64, torch.bfloat16, False),
     (2_100_001, 64, torch.float16, True), (1_050_011, 128, torch.bfloat16, False), (525_001, 256, torch.float16, False),
     (262_151, 512, torch.bfloat16, False), (350_003, 384, torch.bfloat16, True), (131_101, 1024, torch.bfloat16, True),
-    (66_001, 2048, torch.float16, False), (33_001, 2048, torch.float32, True), (16_800, 8192, torch.bfloat16, False)])
+    (66_001, 2048, torch.float16, False), (33_001, 2048, torch.float32, True), (16_800, 8192, torch.bfloat16, False),
+    (8_300, 8192, torch.float32, False), (4_300, 16_000, torch.float32, True), (8_500, 16_000, torch.bfloat16, True),
+    (8_500, 16_000, torch.float16, False)])
 def test_tables_beyond_the_caches(M, F, dtype, joined):
     """From 256 MB on whole-line tables take the streaming forms: sampled rows against the formulas, the column sums
     against sums over the whole table in float64 on the GPU."""

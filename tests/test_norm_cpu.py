@@ -112,3 +112,14 @@ def test_model_options():
     assert bool((m.norms[1].weight == 1).all())
     with pytest.raises(ValueError, match="GPU"):
         m.train()(torch.randn(5, 7), torch.zeros(2, 3, dtype=torch.int64))
+
+
+def test_a_model_pickled_before_the_options_existed():
+    from graphsage_amd import GraphSAGE
+    m = GraphSAGE()
+    for k in ("norm", "residual", "input_dropout"):
+        del m.__dict__[k]
+    m.reset_parameters()
+    assert (m.norm, m.residual, m.input_dropout) == (None, False, 0.0)
+    with pytest.raises(ValueError, match="GPU"):
+        m.train()(torch.randn(5, 7), torch.zeros(2, 3, dtype=torch.int64))
