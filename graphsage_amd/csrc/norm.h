@@ -30,15 +30,17 @@ struct NormBwd {
 };
 
 // Which kernel a row takes: K vectors of 16 bytes (V elements each) in each of R lanes of a wave, or of `row` threads of a
-// workgroup (B); NORM_ONE: rows shorter than a vector, an element a lane.  A row's sums and addresses cost its threads the
-// same whatever they hold, so a row takes the fewest lanes that need no more than three vectors each, which also leaves
-// few of them idle (fp16 240 000 x 264, joined: 16 lanes x 3 78 us forward and 135 backward, 32 x 2 92 and 167).  Two or
-// four waves a row rather than three or five: eight fit a compute unit.  Past 8192 columns (NORM_W) 16 elements a thread in
-// up to sixteen waves, as many as a compute unit has room for: 8192 x 16000 bf16 forward 97 us, backward 176, joined 143
-// and 304; as eight waves with 32 elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).
-// Large fp32 tables of whole cache lines without residual or dropout stream best where neighbouring lanes hold
-// neighbouring vectors (`stream`: 10 M x 64 forward 0.81 ms at 16 lanes x 1, 0.85 at 8 x 2, backward 1.25 and 1.34; 4 M x
-// 128 0.65 and 0.68, 1.01 and 1.08; bf16 2 M x 256 0.325 and 0.319, 0.548 and 0.541).
+// workgroup (B, W); NORM_ONE: rows shorter than a vector, an element a lane.  A row's sums and addresses cost its threads
+// the same whatever they hold, so a row takes the fewest lanes that need no more than three vectors each, which also
+// leaves few of them idle (fp16 240 000 x 264, joined: 16 lanes x 3 78 us forward and 135 backward, 32 x 2 92 and 167).
+// Past a vector each of four lanes at least eight: a wave's accesses then take whole lines (4 M x 64 bf16 forward 0.167
+// ms, at four lanes x 2 0.220).  Two or four waves a row rather than three or five: eight fit a compute unit (40 000 x 1544
+// fp16 joined forward 79 us, 80).  Past 8192 columns (NORM_W) 16 elements a thread in up to sixteen waves, as many as a
+// compute unit has room for: 8192 x 16000 bf16 forward 97 us, backward 176, joined 143 and 304; as eight waves with 32
+// elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).  Large fp32 tables of whole cache
+// lines without residual or dropout stream best where neighbouring lanes hold neighbouring vectors (`stream`: 10 M x 64
+// forward 0.81 ms at 16 lanes x 1, 0.85 at 8 x 2, backward 1.25 and 1.34; 4 M x 128 0.65 and 0.68, 1.01 and 1.08; bf16
+// 2 M x 256 0.325 and 0.319, 0.548 and 0.541).
 enum NormKind { NORM_ONE, NORM_R4, NORM_R8, NORM_R8x2, NORM_R8x3, NORM_R16, NORM_R16x2, NORM_R16x3, NORM_R32, NORM_R32x2,
                 NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_W, NORM_LONG };
 struct NormForm { NormKind kind; int row; };      // threads of a row

@@ -11,6 +11,9 @@ backward draws it again.  A dropped element gives exactly 0, forward and backwar
 ``seed`` is an int, a one-element int64 tensor on the device (read when the kernel runs: a captured graph that
 rewrites it draws other masks on each replay, where an int is frozen into the graph), or None: one draw from
 torch's CPU generator.
+
+A backward is captured into a graph like any other of torch's: with no eager graph of the same leaves alive, whose
+gradient nodes torch would run on the stream they were made on.
 """
 from __future__ import annotations
 
