@@ -35,14 +35,16 @@ struct NormBwd {
 // leaves few of them idle (fp16 240 000 x 264, joined: 16 lanes x 3 78 us forward and 135 backward, 32 x 2 92 and 167).
 // Past a vector each of four lanes at least eight: a wave's accesses then take whole lines (4 M x 64 bf16 forward 0.167
 // ms, at four lanes x 2 0.220).  Two or four waves a row rather than three or five: eight fit a compute unit (40 000 x 1544
-// fp16 joined forward 79 us, 80).  Past 8192 columns (NORM_W) 16 elements a thread in up to sixteen waves, as many as a
+// fp16 joined forward 79 us, 80); where that would be three or four waves of three vectors, nine to twelve of one (NORM_W1:
+// 8191 x 5120 bf16 joined with its sum forward 65 us, backward 112; in fours 66 and 122; 9000 x 2600 fp32 34 and 61, joined
+// 51 and 91; 36 and 62, 54 and 94).  Past 8192 columns (NORM_W) 16 elements a thread in up to sixteen waves, as many as a
 // compute unit has room for: 8192 x 16000 bf16 forward 97 us, backward 176, joined 143 and 304; as eight waves with 32
 // elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).  Large fp32 tables of whole cache
 // lines without residual or dropout stream best where neighbouring lanes hold neighbouring vectors (`stream`: 10 M x 64
 // forward 0.81 ms at 16 lanes x 1, 0.85 at 8 x 2, backward 1.25 and 1.34; 4 M x 128 0.65 and 0.68, 1.01 and 1.08; bf16
 // 2 M x 256 0.325 and 0.319, 0.548 and 0.541).
 enum NormKind { NORM_ONE, NORM_R4, NORM_R8, NORM_R8x2, NORM_R8x3, NORM_R16, NORM_R16x2, NORM_R16x3, NORM_R32, NORM_R32x2,
-                NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_W, NORM_LONG };
+                NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_W1, NORM_W, NORM_LONG };
 struct NormForm { NormKind kind; int row; };      // threads of a row
 static inline NormForm norm_form(int64_t F, int V, bool stream) {
   stream = stream && V == 4;
@@ -65,7 +67,7 @@ static inline NormForm norm_form(int64_t F, int V, bool stream) {
   if (nv <= 256) return {NORM_B2, 128};
   if (nv <= 384) return {NORM_B3, 128};
   if (nv <= 512) return {NORM_B2, 256};
-  if (nv <= 768) return {NORM_B3, waves(3)};
+  if (nv <= 768) return {NORM_W1, waves(1)};
   if (nv <= 1024) return {NORM_B2, waves(2)};
   if (nv <= 2048 && V == 4) return {NORM_B4, waves(4)};
   if (nv <= 16384 / V) return {NORM_W, waves(16 / V)};

@@ -214,10 +214,10 @@ template <typename T> struct Ln {
   NormDrop d;
 };
 
-// A row takes TPR lanes of a wave, or a.row threads: up to 8 (TPR = 0) or 16 (TPR = -1) whole waves.  A workgroup takes as many rows at
-// once as fit.  Thread t of the row holds K vectors of V columns, a row's threads apart.  A vector that would go past the
-// row's end is moved back to end with it; its first `lo` elements (all of them, where the thread has nothing left to do)
-// then belong to vectors before it: both threads form and store the same values, the sums count them once.
+// A row takes TPR lanes of a wave, or a.row threads: up to 8 (TPR = 0) or 16 (TPR = -1) whole waves.  A workgroup takes as
+// many rows at once as fit.  Thread t of the row holds K vectors of V columns, a row's threads apart.  A vector that would
+// go past the row's end is moved back to end with it; its first `lo` elements (all of them, where the thread has nothing
+// left to do) then belong to vectors before it: both threads form and store the same values, the sums count them once.
 constexpr int MAXW = 8;
 constexpr int ln_waves(int TPR) { return TPR < 0 ? 16 : MAXW; }
 template <int V, int TPR, int K> struct Cols {
@@ -409,11 +409,10 @@ constexpr int FLUSH = 16;
 
 // Workgroups of eight waves (fewer slabs than four would leave), or of the row's up to sixteen.  The row after is loaded a
 // row ahead where there are registers for it: not at 24 elements a thread (fp16 257 columns 39 us, joined 71; with four
-// waves that have them 42 and 83; 6000 columns joined 212 and 217), nor at 16 of fp32 joined, nor of sixteen waves, which
-// have 128 each; those read grad_sum, too, only when the weights are used up (fp32 8192 x 16000 joined 661 us; with the
+// waves that have them 42 and 83), nor at 16 of fp32 joined, nor at 16 in sixteen waves, which have 128 each; those read grad_sum, too, only when the weights are used up (fp32 8192 x 16000 joined 661 us; with the
 // other operands 758).
 constexpr bool ln_bwd_ahead(int V, int TPR, int K, bool JOIN) {
-  return TPR >= 0 && K * V < 24 && !(JOIN && K * V == 16 && V == 4);
+  return (TPR >= 0 || K == 1) && K * V < 24 && !(JOIN && K * V == 16 && V == 4);
 }
 constexpr int ln_bwd_threads(int TPR) { return 64 * ln_waves(TPR); }
 
@@ -425,6 +424,7 @@ __device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g, Grads<T> d) {
   constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
+  constexpr bool LATE = TPR < 0 && !AHEAD;      // grad_sum is read when the weights are used up
   constexpr int A = AHEAD ? K : 1;
   extern __shared__ float acc[];              // [2 K V][threads]: grad_w, then grad_b; a thread's words are its own
   constexpr int WAVES = ln_waves(TPR);
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
     next.load(a, c, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) gnext[k].template load<NT>(d.g + r * a.F + c.col[k]);
-    if (JOIN && d.gsum && TPR >= 0)
+    if (JOIN && d.gsum && !LATE)
 #pragma unroll
       for (int k = 0; k < K; ++k) snext[k].template load<NT>(d.gsum + r * a.F + c.col[k]);
     mnext = d.mean[r];
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       gnext[k].open(gv[k]);
-      if (JOIN && TPR >= 0) sv[k] = snext[k];
+      if (JOIN && !LATE) sv[k] = snext[k];
     }
     const float m = mnext, rs = rnext;
     if (AHEAD && turn + 1 < g.turns) fetch(row + g.step);
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
         }
         gv[k][i] *= w[k][i];
       }
-    if (JOIN && TPR < 0 && d.gsum)
+    if (JOIN && LATE && d.gsum)
 #pragma unroll
       for (int k = 0; k < K; ++k) sv[k].template load<NT>(d.gsum + (row < a.M ? row : a.M - 1) * a.F + c.col[k]);
     if (a.F % V == 0) {                     // (g is zero where a thread has no column)
@@ -799,7 +799,7 @@ constexpr int64_t MAX_GRID = 1 << 20;      // workgroups of a launch (a launch's
 // Workgroups of this kernel that the GPU holds at once: the rows are dealt out to these, none waits for a place
 template <auto KERNEL> int ln_resident(int threads, int lds) {
   static std::atomic<int> known[16 + 1];
-  if (lds > 65536) {      // (the attribute is a device's own)
+  if (lds >= 65536) {      // (the kernels have a little LDS of their own besides; the attribute is a device's own)
     static std::atomic<bool> done[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
@@ -837,9 +837,9 @@ void ln_fwd_launch(const Ln<T> &a, int turns, float eps, T *y, T *sum, float *me
 
 // One turn a workgroup, where it has 3200 bytes of rows to spread its weights over (fp32 2 M x 28: 81 us, 83 as a loop of
 // two turns; 2 M x 20: 70 us, as a loop 60; 4 M x 4 59 and 41); 16-bit rows without dropout or a residual need two (less
-// arithmetic a byte: 4 M x 64 bf16 0.167 against 0.181 ms), and so do rows of two or four waves.  Rows of
-// several waves with three vectors a thread or more, and of more than eight waves, run as loops over the grid that the GPU
-// holds (8191 x 5120 bf16 33 us, 42 in order).
+// arithmetic a byte: 4 M x 64 bf16 0.167 against 0.181 ms), and so do rows of two or four waves.  Rows of several waves
+// with three vectors a thread or more, and of more than eight waves, run as loops over the grid that the GPU holds (8191 x
+// 5120 bf16 in three waves 33 us, 42 in order).
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd, hipStream_t st) {
   const int64_t bytes = 256 / (TPR > 0 ? TPR : 256) * (int64_t)a.F * sizeof(T);
@@ -885,7 +885,7 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   CASE(NORM_R8x3, V, 8, 3) LINE(NORM_R16, V, 16, 1) CASE(NORM_R16x2, V, 16, 2) CASE(NORM_R16x3, V, 16, 3)     \
   LINE(NORM_R32, V, 32, 1) CASE(NORM_R32x2, V, 32, 2) CASE(NORM_R32x3, V, 32, 3) LINE(NORM_R64, V, 64, 1)     \
   CASE(NORM_R64x2, V, 64, 2) CASE(NORM_R64x3, V, 64, 3) CASE(NORM_B2, V, 0, 2) CASE(NORM_B3, V, 0, 3)                          \
-  CASE(NORM_W, V, -1, 16 / V)
+  CASE(NORM_W1, V, -1, 1) CASE(NORM_W, V, -1, 16 / V)
 
 template <typename T>
 int ln_fwd(const NormFwd &n, hipStream_t st) {
