@@ -70,9 +70,9 @@ def test_layer_norm_forward_backward(M, F, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,F", [(700, 8201), (600, 12_347), (530, 16_384), (520, 16_500)])
+@pytest.mark.parametrize("M,F", [(900, 2571), (800, 5003), (700, 8201), (600, 12_347), (530, 16_384), (520, 16_500)])
 def test_wide_rows_by_the_workgroup(M, F, dtype):
-    """rows of sixteen waves and longer, several of them a workgroup"""
+    """rows of nine to sixteen waves and longer, several of them a workgroup"""
     c, g, gsum = _case(M, F, dtype, M + F, wdtype=torch.float32 if F % 2 else None, with_sum=F % 4 == 0)
     _run(c, g, gsum, 0.3, F, f"{M}x{F} {dtype}")
 
