@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(TPR > 0 || K == 3 ? 256 : 64 * ln_waves(TPR)) 
       // (waves that are not there have no elements; their slots hold whatever LDS held)
       const float so = other ? slot[threadIdx.x % WAVES][0] : 0.f, qo = other ? slot[threadIdx.x % WAVES][1] : 0.f;
       m = lanes_sum<WAVES>(so) * inv_f;
-      const float e = so * inv_other - m;
+      const float e = other ? so * inv_other - m : 0.f;      // (m^2 times no elements: a mean past 2^64 would make it NaN)
       var = lanes_sum<WAVES>(fmaf(e * e, (float)other, qo)) * inv_f;
     }
     const float rs = rsqrtf(var + eps);
@@ -682,8 +682,8 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_k(Ln<T> a, float eps, T *y, 
       const float nv = (float)(V - at.lo), mv = s / nv;
 #pragma unroll
       for (int i = 0; i < V; ++i) { const float e = i >= at.lo ? z[i] - mv : 0.f; qv = fmaf(e, e, qv); }
-      const float all = n + nv, e = mv - m;
-      m = fmaf(e, nv / all, m);
+      const float all = n + nv, e = n > 0.f ? mv - m : 0.f;      // (the first vector's mean is no distance from another)
+      m = n > 0.f ? fmaf(e, nv / all, m) : mv;
       q += fmaf(e * e, n * nv / all, qv);
       n = all;
     }

@@ -1,0 +1,34 @@
+"""GPU: layer norm at the ends of fp32's range: rows whose values, though finite, are so large that a square of the mean or
+a product with 1 / sigma is not."""
+import pytest
+import torch
+
+import graphsage_amd as gs
+
+import norm_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+# rows of two waves to sixteen that leave some of a workgroup's waves without elements, one that does not, and rows
+# longer than a workgroup's registers (fp32 and 16 bits take other kernels at the same width)
+LARGE = [(torch.float32, F) for F in (200, 900, 1500, 2000, 2500, 3400, 6000, 10_000, 16_384, 16_385, 40_000)] + \
+        [(torch.bfloat16, F) for F in (1000, 1800, 3000, 4000, 5000, 7000, 9000, 20_000)]
+
+
+@pytest.mark.parametrize("joined", [False, True])
+@pytest.mark.parametrize("dtype,F", LARGE)
+def test_means_whose_square_passes_the_range(dtype, F, joined):
+    """Rows of 2^65, an element in 64 larger by 2^58: mean^2 = 2^130 is no fp32 number, the squares about the mean (2^116
+    each, 2^126 in all) are."""
+    gen = torch.Generator().manual_seed(F)
+    x = torch.full((5, F), 2.0 ** 65)
+    x[torch.rand(5, F, generator=gen) < 1 / 64] *= 1 + 2.0 ** -7
+    x = x.to(dtype)
+    residual = torch.zeros(5, F, dtype=dtype) if joined else None
+    w, g = (1 + 0.2 * torch.randn(F, generator=gen)).to(dtype), torch.randn(5, F, generator=gen).to(dtype)
+    want = ref.reference(x, residual, w, g=g)
+    d = [t.cuda().requires_grad_() for t in (x, w)]
+    y = gs.dropout_add_layer_norm(d[0], residual.cuda() if joined else None, d[1])
+    ref.check(y, want["y"], f"{F} {dtype} y")
+    for got, name in zip(torch.autograd.grad(y, d, g.cuda()), ("grad_x", "grad_weight")):
+        ref.check(got, want[name], f"{F} {dtype} {name}")
