@@ -496,10 +496,11 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
     if (AHEAD && turn % FLUSH == FLUSH - 1) flush();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+      const float mk = c.on[k] ? m : 0.f;      // h = 0 without a column: m rs may pass the range, and g = 0 times that is NaN
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        h[k][i] = (h[k][i] - m) * rs;
+        h[k][i] = (h[k][i] - mk) * rs;
         if constexpr (AHEAD) {
           dw[k][i] = fmaf(gv[k][i], h[k][i], dw[k][i]);
           db[k][i] += gv[k][i];
@@ -509,6 +510,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
         }
         gv[k][i] *= w[k][i];
       }
+    }
     if (JOIN && LATE && d.gsum)
 #pragma unroll
       for (int k = 0; k < K; ++k) sv[k].template load<NT>(d.gsum + (row < a.M ? row : a.M - 1) * a.F + c.col[k]);

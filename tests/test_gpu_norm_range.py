@@ -32,3 +32,26 @@ def test_means_whose_square_passes_the_range(dtype, F, joined):
     ref.check(y, want["y"], f"{F} {dtype} y")
     for got, name in zip(torch.autograd.grad(y, d, g.cuda()), ("grad_x", "grad_weight")):
         ref.check(got, want[name], f"{F} {dtype} {name}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("F", [2, 4, 8, 16, 20, 24, 40, 72, 100, 200, 300, 700])
+def test_constant_rows_whose_mean_over_sigma_passes_the_range(F, dtype):
+    """Rows of one number c have h = 0 and sigma = sqrt(eps) whatever c is, so their gradients are those of c = 0, bit for
+    bit; at c = 2^110 and eps = 1e-12, c / sigma is no fp32 number."""
+    c = 2.0 ** 110
+    one = torch.ones((), dtype=torch.float32)
+    assert float(F * one * (one / F)) == 1.0        # (so that the kernel's mean of F numbers c is c)
+    gen = torch.Generator().manual_seed(F)
+    w, g = (1 + 0.2 * torch.randn(F, generator=gen)).to(dtype).cuda(), torch.randn(9, F, generator=gen).to(dtype).cuda()
+    res = torch.zeros(9, F, dtype=dtype, device="cuda")
+    outs = []
+    for value in (0.0, c):
+        x = torch.full((9, F), value, dtype=dtype, device="cuda").requires_grad_()
+        wl = w.clone().requires_grad_()
+        plain = torch.autograd.grad(gs.layer_norm(x, wl, eps=1e-12), [x, wl], g)
+        joined = torch.autograd.grad(gs.dropout_add_layer_norm(x, res, wl, eps=1e-12), [x, wl], g)
+        outs.append([*plain, *joined])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and bool(torch.isfinite(b).all())
+    assert float(outs[0][0].abs().max()) > 0
