@@ -35,13 +35,13 @@ def test_means_whose_square_passes_the_range(dtype, F, joined):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("F", [2, 4, 8, 16, 20, 24, 40, 72, 100, 200, 300, 700])
+@pytest.mark.parametrize("F", [2, 4, 8, 16, 32, 64, 256, 1024])
 def test_constant_rows_whose_mean_over_sigma_passes_the_range(F, dtype):
     """Rows of one number c have h = 0 and sigma = sqrt(eps) whatever c is, so their gradients are those of c = 0, bit for
-    bit; at c = 2^110 and eps = 1e-12, c / sigma is no fp32 number."""
+    bit; at c = 2^110 and eps = 1e-12, c / sigma is no fp32 number.  Widths whose 1 / F is exact: of another the kernel takes
+    c - (c F) fl(1 / F), fused, which is c d, |d| <= 2^-24 the rounding of 1 / F; (c d)^2 = 2^172 is infinite, 1 / sigma 0,
+    and so are the gradients, within what fp32 means allow (an error of L u c in the mean against sigma = 2^-20)."""
     c = 2.0 ** 110
-    one = torch.ones((), dtype=torch.float32)
-    assert float(F * one * (one / F)) == 1.0        # (so that the kernel's mean of F numbers c is c)
     gen = torch.Generator().manual_seed(F)
     w, g = (1 + 0.2 * torch.randn(F, generator=gen)).to(dtype).cuda(), torch.randn(9, F, generator=gen).to(dtype).cuda()
     res = torch.zeros(9, F, dtype=dtype, device="cuda")
