@@ -756,14 +756,8 @@ __global__ void __launch_bounds__(1024) ln_dz_long_k(Ln<T> a, const T *g, const 
   }
 }
 
-// acc + v with the error carried on
-__device__ __forceinline__ void add_carry(float &acc, float &carry, float v) {
-  const float y = v - carry, t = acc + y;
-  carry = (t - acc) - y;
-  acc = t;
-}
-
-// A vector of columns a thread, rows blockIdx.y, blockIdx.y + gridDim.y, ... -> slab blockIdx.y
+// A vector of columns a thread, rows blockIdx.y, blockIdx.y + gridDim.y, ... -> slab blockIdx.y.  Summed in double: an fp32
+// sum with its error carried along costs the same registers, and an infinite gradient leaves NaN in the carry.
 template <typename T>
 __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const float *mean, const float *rstd, float *ws) {
   constexpr int V = Tab<T>::V;
@@ -772,7 +766,8 @@ __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const f
   const LongVec<T> at(v, a.F);
   const uint64_t key = drop_key(a.d);
   const uint32_t thr = dropout_threshold(a.d.p);
-  float dw[V] = {}, db[V] = {}, dwc[V] = {}, dbc[V] = {}, h[V], e[V];
+  double dw[V] = {}, db[V] = {};
+  float h[V], e[V];
   bool kept[V];
   for (int64_t r = blockIdx.y; r < a.M; r += gridDim.y) {
     Raw<T, V> gr;
@@ -782,16 +777,16 @@ __global__ void __launch_bounds__(256) ln_dw_long_k(Ln<T> a, const T *g, const f
     const float m = mean[r], rs = rstd[r];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      add_carry(dw[i], dwc[i], e[i] * ((h[i] - m) * rs));
-      add_carry(db[i], dbc[i], e[i]);
+      dw[i] += (double)(e[i] * ((h[i] - m) * rs));
+      db[i] += (double)e[i];
     }
   }
   float *slab = ws + (int64_t)blockIdx.y * 2 * a.F;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (i < at.lo) continue;
-    slab[at.c + i] = dw[i];
-    slab[a.F + at.c + i] = db[i];
+    slab[at.c + i] = (float)dw[i];
+    slab[a.F + at.c + i] = (float)db[i];
   }
 }
 

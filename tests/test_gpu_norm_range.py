@@ -55,3 +55,24 @@ def test_constant_rows_whose_mean_over_sigma_passes_the_range(F, dtype):
     for a, b in zip(*outs):
         assert torch.equal(a, b) and bool(torch.isfinite(b).all())
     assert float(outs[0][0].abs().max()) > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,F", [(600, 6), (5000, 64), (600, 300), (600, 5000), (600, 12_000), (600, 20_000), (5, 40_000)])
+def test_an_infinite_gradient_stays_infinite_in_its_column(M, F, dtype):
+    """One gradient of +inf: its column's grad_bias is +inf and grad_weight the infinity of h's sign; the other columns are
+    what they are without it, bit for bit."""
+    gen = torch.Generator().manual_seed(F)
+    x = torch.randn(M, F, generator=gen).to(dtype).cuda()
+    w = torch.ones(F, dtype=dtype, device="cuda", requires_grad=True)
+    b = torch.zeros(F, dtype=dtype, device="cuda", requires_grad=True)
+    g = torch.randn(M, F, generator=gen).to(dtype).cuda()
+    y = gs.layer_norm(x, w, b)
+    clean = torch.autograd.grad(y, [w, b], g, retain_graph=True)
+    row, col, inf = M // 7, F // 2, float("inf")
+    g[row, col] = inf
+    gw, gb = torch.autograd.grad(y, [w, b], g)
+    h = float(y.detach()[row, col])             # (weight one, bias zero)
+    assert h != 0.0 and float(gb[col]) == inf and float(gw[col]) == (inf if h > 0 else -inf)
+    rest = torch.arange(F, device="cuda") != col
+    assert torch.equal(gw[rest], clean[0][rest]) and torch.equal(gb[rest], clean[1][rest])
