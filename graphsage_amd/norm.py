@@ -12,6 +12,9 @@ backward draws it again.  A dropped element gives exactly 0, forward and backwar
 rewrites it draws other masks on each replay, where an int is frozen into the graph), or None: one draw from
 torch's CPU generator.
 
+Derivatives are reverse mode, once: forward mode raises ``NotImplementedError``, a second derivative ``RuntimeError``.
+``torch.jit.trace`` records a call as a Python function (an int or drawn seed frozen into it).
+
 A backward is captured into a graph like any other of torch's: with no eager graph of the same leaves alive, whose
 gradient nodes torch would run on the stream they were made on.
 """
@@ -21,6 +24,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -102,7 +106,7 @@ def _call(tag: str, device: torch.device, entry, *args) -> None:
 def _dropout(x: torch.Tensor, p: float, seed) -> torch.Tensor:
     value, pointer = _split(seed)
     out = torch.empty_like(x)
-    _call("dropout", x.device, _lib.load().gsage_dropout, x.data_ptr(), x.numel(), _DTYPES[x.dtype], p, value, pointer,
+    _call("dropout", x.device, _lib.load().gsage_dropout, x.data_ptr(), int(x.numel()), _DTYPES[x.dtype], p, value, pointer,
           out.data_ptr())
     return out
 
@@ -110,8 +114,8 @@ def _dropout(x: torch.Tensor, p: float, seed) -> torch.Tensor:
 def layer_norm_fwd(x, residual, weight, bias, eps: float, p: float, seed, want_sum: bool, want_stats: bool):
     """gsage_layer_norm_fwd on contiguous operands -> (y, sum or None, [mean, rstd] as fp32 [2, M] or None)."""
     value, pointer = _split(seed)
-    F = x.size(-1)
-    M = x.numel() // F
+    F = int(x.size(-1))           # (sizes are tensors while torch.jit.trace records)
+    M = int(x.numel()) // F
     y = torch.empty_like(x)
     total = torch.empty_like(x) if want_sum else None
     stats = mean = rstd = None
@@ -132,8 +136,8 @@ def layer_norm_bwd(grad_y, grad_sum, x, residual, weight, stats, p: float, seed,
     lib = _lib.load()
     value, pointer = _split(seed)
     dev, code = x.device, _DTYPES[x.dtype]
-    F = x.size(-1)
-    M = x.numel() // F
+    F = int(x.size(-1))
+    M = int(x.numel()) // F
     gx = torch.empty_like(x) if need[0] else None
     gres = torch.empty_like(x) if need[1] else None
     gw = torch.empty(F, dtype=wdtype, device=dev) if need[2] else None
@@ -169,6 +173,12 @@ def _once(backward):
     def call(ctx, *grads):
         return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return call
+
+
+def _watched() -> bool:
+    """Whether torch has to see the call though no gradient is wanted: a launch on raw pointers would give an output
+    without a tangent in forward mode (through the function it raises) and leave the kernel out of a trace."""
+    return forward_ad._current_level >= 0 or torch._C._is_tracing()
 
 
 class DropoutFunction(torch.autograd.Function):
@@ -222,7 +232,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, seed: Seed =
     if not training or p == 0.0:
         return x
     seed = _seed(seed, x.device)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if (torch.is_grad_enabled() and x.requires_grad) or _watched():
         return DropoutFunction.apply(x, p, seed)
     return _dropout(x, p, seed)
 
@@ -256,9 +266,9 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
     if not training:
         p = 0.0
     seed = _seed(seed, x.device) if p > 0.0 else 0
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad) or
-                                    (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad) or
+                                     (weight is not None and weight.requires_grad) or
+                                     (bias is not None and bias.requires_grad))) or _watched():
         return LayerNormFunction.apply(x, residual, weight, bias, eps, p, seed, return_sum)
     y, total, _ = layer_norm_fwd(x, residual, weight, bias, eps, p, seed, return_sum, False)
     return (y, total) if return_sum else y
