@@ -402,10 +402,18 @@ template <typename T> struct Grads {
 };
 
 // ------------------------------------------------------------------ backward
-// A thread's column sums: in registers for 16 rows, then added to its own words of LDS (of thousands of rows in a row an
-// fp32 sum would lose some bits, and the registers of a second level would cost occupancy).  Where there are no registers
-// for the first level either every row goes to LDS.
-constexpr int FLUSH = 16;
+// A thread's column sums: in registers for `flush` rows, then added in double to its own words of LDS, which so hold
+// thousands of rows without losing bits (fp32 words: 33 M rows x 64 of one gradient off by 24 roundings, doubles by none).
+// Doubles cost a flush 0.8 us where a thread has 16 elements, so they come from `doubles` rows a thread on (fewer stay in
+// registers to the end), rows that share waves with others flush a wave at a time (`late`; 1 M x 196 fp16 208 us, all at
+// once 215, in fp32 words 207) and rows of several waves half as often (40 000 x 1544 fp16 72 us, every 16 rows 75, in
+// fp32 words 72).  Joined rows that share a wave have neither: tests of the turn's number beside the loop's own cost more there
+// (4 M x 3 fp32 82 us, 116 to 120 with them; the doubles themselves 1 to 2 %).
+// Where there are no registers for the first level (ln_bwd_ahead) every row goes to LDS, in fp32: two words for each of 24
+// elements, or of 16 in sixteen waves, do not fit there.  A thread's sum of n rows of either sign is then off by some
+// sqrt(n) / 2.4 roundings: 6 at the 200 rows of 3 M x 192 bf16.
+constexpr int ln_bwd_flush(int TPR) { return TPR > 0 ? 16 : 32; }
+constexpr int ln_bwd_doubles(int TPR, bool JOIN) { return TPR > 0 && JOIN ? 16 : 2 * ln_bwd_flush(TPR); }
 
 // Workgroups of eight waves (fewer slabs than four would leave), or of the row's up to sixteen.  The row after is loaded a
 // row ahead where there are registers for it: not at 24 elements a thread (fp16 257 columns 39 us, joined 71; with four
@@ -424,13 +432,14 @@ __device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g, Grads<T> d) {
   constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
+  constexpr int FLUSH = ln_bwd_flush(TPR), DOUBLES = ln_bwd_doubles(TPR, JOIN);
   constexpr bool LATE = TPR < 0 && !AHEAD;      // grad_sum is read when the weights are used up
   constexpr int A = AHEAD ? K : 1;
-  extern __shared__ float acc[];              // [2 K V][threads]: grad_w, then grad_b; a thread's words are its own
+  // [2 K V][threads] column sums: grad_w, then grad_b; a thread's words are its own.  Doubles where registers come first
+  extern __shared__ __attribute__((aligned(8))) char lds[];
   constexpr int WAVES = ln_waves(TPR);
   __shared__ float part[TPR > 0 ? 1 : 2][TPR > 0 ? 1 : WAVES][2];
   constexpr int threads = ln_bwd_threads(TPR);      // (a workgroup a row may have fewer)
-  float *const mine = acc + threadIdx.x;
   const Cols<V, TPR, K> c(a.F, a.row);
   const int rows = TPR > 0 ? threads / (TPR > 0 ? TPR : 1) : blockDim.x / c.threads, first = TPR < 0 ? 0 : threadIdx.x / c.threads;
   int64_t base = g.begin + (int64_t)blockIdx.x * g.apart, row = base + first;
@@ -451,6 +460,7 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
   fetch(row);
   Weights<T, V> wr[K];
   float w[K][V], dw[A][V], db[A][V];
+  float *const mine = (float *)lds + threadIdx.x;      // (without registers for them)
 #pragma unroll
   for (int k = 0; k < K; ++k) wr[k].load(a.w, a.wdtype, c.col[k]);
 #pragma unroll
@@ -458,21 +468,25 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if (AHEAD) dw[k % A][i] = db[k % A][i] = 0.f;
-      mine[(k * V + i) * threads] = mine[((K + k) * V + i) * threads] = 0.f;
+      else mine[(k * V + i) * threads] = mine[((K + k) * V + i) * threads] = 0.f;
     }
     wr[k].open(a.w, a.wdtype, 1.f, w[k]);
   }
   const uint64_t key = JOIN ? drop_key(a.d) : 0;
   const uint32_t thr = JOIN ? dropout_threshold(a.d.p) : 0;
   const float inv_f = 1.0f / (float)a.F;
-  const auto flush = [&]() {
+  const bool doubles = g.turns >= DOUBLES;      // (every wave has flushed by then)
+  const int late = TPR > 0 && !JOIN ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const auto flush = [&](auto *sums, bool first) {      // (the first one writes, for there is nothing to add to)
     if constexpr (AHEAD) {
+      sums += threadIdx.x;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          mine[(k * V + i) * threads] += dw[k][i];
-          mine[((K + k) * V + i) * threads] += db[k][i];
+          auto &uw = sums[(k * V + i) * threads], &ub = sums[((K + k) * V + i) * threads];
+          uw = first ? dw[k][i] : uw + dw[k][i];
+          ub = first ? db[k][i] : ub + db[k][i];
           dw[k][i] = db[k][i] = 0.f;
         }
     }
@@ -493,7 +507,10 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
     }
     const float m = mnext, rs = rnext;
     if (AHEAD && turn + 1 < g.turns) fetch(row + g.step);
-    if (AHEAD && turn % FLUSH == FLUSH - 1) flush();
+    if (AHEAD && (DOUBLES == FLUSH || doubles)) {
+      const int since = turn + 1 - late;
+      if (since > 0 && since % FLUSH == 0) flush((double *)lds, since == FLUSH);
+    }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -564,23 +581,31 @@ __global__ void __launch_bounds__(ln_bwd_threads(TPR)) ln_bwd_k(Ln<T> a, Walk g,
     if constexpr (NT) settle();
   }
   if (!d.ws) return;
-  flush();
-  __syncthreads();
   // this workgroup's column sums -> its slab, or (one workgroup) the result: element e of thread t's columns, over the
   // threads of the workgroup's rows that hold the same columns (up to 128: in double)
-  float *slab = d.ws + (int64_t)blockIdx.x * 2 * a.F;
-  for (int j = threadIdx.x; j < K * V * c.threads; j += blockDim.x) {
-    const int t = j % c.threads, e = j / c.threads, v = (t + e / V * c.threads) * V, at = v < a.F - V ? v : a.F - V;
-    if (v >= a.F || e % V < v - at) continue;
-    double u = 0., q = 0.;
-    for (int r = 0; r < rows; ++r) {
-      u += acc[e * threads + r * c.threads + t];
-      q += acc[(K * V + e) * threads + r * c.threads + t];
+  const auto finish = [&](const auto *sums) {
+    __syncthreads();
+    float *slab = d.ws + (int64_t)blockIdx.x * 2 * a.F;
+    for (int j = threadIdx.x; j < K * V * c.threads; j += blockDim.x) {
+      const int t = j % c.threads, e = j / c.threads, v = (t + e / V * c.threads) * V, at = v < a.F - V ? v : a.F - V;
+      if (v >= a.F || e % V < v - at) continue;
+      double u = 0., q = 0.;
+      for (int r = 0; r < rows; ++r) {
+        u += sums[e * threads + r * c.threads + t];
+        q += sums[(K * V + e) * threads + r * c.threads + t];
+      }
+      const int col = at + e % V;
+      if (gridDim.x > 1) { slab[col] = (float)u; slab[a.F + col] = (float)q; continue; }
+      if (d.gw) store_w(d.gw, a.wdtype, col, (float)u);
+      if (d.gb) store_w(d.gb, a.wdtype, col, (float)q);
     }
-    const int col = at + e % V;
-    if (gridDim.x > 1) { slab[col] = (float)u; slab[a.F + col] = (float)q; continue; }
-    if (d.gw) store_w(d.gw, a.wdtype, col, (float)u);
-    if (d.gb) store_w(d.gb, a.wdtype, col, (float)q);
+  };
+  if (AHEAD && doubles) {
+    flush((double *)lds, false);
+    finish((const double *)lds);
+  } else {      // (the registers' sums as they are)
+    flush((float *)lds, true);
+    finish((const float *)lds);
   }
 }
 
@@ -853,7 +878,8 @@ void ln_fwd_go(const Ln<T> &a, float eps, T *y, T *sum, float *mean, float *rstd
 template <typename T, int V, int TPR, int K, bool JOIN, bool NT>
 int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   constexpr auto kernel = ln_bwd_k<T, V, TPR, K, JOIN, NT>;
-  constexpr int lds = 2 * K * V * ln_bwd_threads(TPR) * (int)sizeof(float);
+  constexpr bool AHEAD = ln_bwd_ahead(V, TPR, K, JOIN);
+  constexpr int few = 2 * K * V * ln_bwd_threads(TPR) * (int)sizeof(float), lds = AHEAD ? 2 * few : few;
   const int rows = ln_bwd_threads(TPR) / a.row, threads = rows * a.row, resident = ln_resident<kernel>(threads, lds);
   // Streamed fp32 tables of short rows in order, as the forward takes them, two turns a workgroup and a slab for each:
   // 10 M x 64 1.37 -> 1.25 ms, 4 M x 128 1.06 -> 1.01 (joined, and in 16 bits, nothing is gained: more arithmetic a byte).
@@ -861,7 +887,9 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   constexpr int turns = 2;
   if (NT && !JOIN && d.ws && norm_folds(a.M, a.F, sizeof(T)) && rows * turns >= NORM_FOLD_ROWS) {
     const int blocks = (int)((a.M + rows * turns - 1) / (rows * turns)), folded = norm_blocks(blocks, 1, 256);
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), lds, st, a, Walk{0, (int64_t)rows * turns, rows, turns}, d);
+    static_assert(!AHEAD || turns < ln_bwd_doubles(TPR, JOIN), "the column sums are fp32 words");
+    // (room for two workgroups a compute unit: 1 M x 96 192 us, 218 with doubles')
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), few, st, a, Walk{0, (int64_t)rows * turns, rows, turns}, d);
     const int per = (blocks + folded - 1) / folded;
     float *out = d.ws + (int64_t)blocks * 2 * a.F;
     hipLaunchKernelGGL(ln_fold_k, dim3((unsigned)((2 * a.F + 63) / 64), folded), dim3(1024), 0, st, d.ws, blocks, per, a.F, out);

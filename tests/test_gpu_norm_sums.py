@@ -80,3 +80,15 @@ def test_in_the_tables_type(F, M, dtype):
 def test_tables_beyond_the_caches_count_every_row_once(M, F, dtype, joined):
     """The streaming forms (256 MB and whole lines), among them the slabs that are folded first (plain fp32, up to 128)."""
     _exact(M, F, dtype, joined, torch.float32)
+
+
+@pytest.mark.parametrize("M,F,joined", [(1 << 25, 64, True), (1 << 25, 64, False), (1 << 25, 130, False), (1 << 22, 770, False)])
+def test_thousands_of_rows_a_thread_lose_no_bits(M, F, joined):
+    """Every gradient is v = 1 + 2^-18: sums of up to 32 are fp32 numbers, and the sum of 16 or 32 of them added to an fp32
+    sum of 64 such or more is half a step past it and lost.  Left are a slab's rounding and the result's: 2 u (+ u^2)."""
+    v = 1.0 + 2.0 ** -18
+    x = torch.zeros(M, F, device="cuda")
+    b = torch.zeros(F, device="cuda", requires_grad=True)
+    y = gs.dropout_add_layer_norm(x, x if joined else None, None, b)
+    gb, = torch.autograd.grad(y, b, torch.full((M, F), v, device="cuda"))
+    assert float((gb.double() - M * v).abs().max()) <= 2.001 * U * M * v
