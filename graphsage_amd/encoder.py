@@ -19,9 +19,10 @@ from .graphsage import GraphSAGE, depth_options
 def model_from_checkpoint(checkpoint: dict, fallback_config: Optional[dict] = None) -> GraphSAGE:
     cfg = checkpoint["config"] if "config" in checkpoint else (fallback_config or {})
     mc, fc = cfg.get("model", {}), cfg.get("features", {})
+    options = {**depth_options(mc), "input_dropout": 0.0}      # no dropout of either kind, whatever mode it is put in
     model = GraphSAGE(in_channels=fc.get("dimensions", 7), hidden_channels=mc.get("hidden_dim", 64),
                       out_channels=mc.get("output_dim", 64), num_layers=mc.get("num_layers", 2),
-                      dropout=0.0, normalize_output=mc.get("normalize_output", True), **depth_options(mc))
+                      dropout=0.0, normalize_output=mc.get("normalize_output", True), **options)
     model.load_state_dict(checkpoint["model_state_dict"])      # strict, PyG key layout
     return model
 
