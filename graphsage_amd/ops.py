@@ -774,9 +774,11 @@ class SAGELayerFunction(torch.autograd.Function):
         # layer's output): the way the two backwards meet in gsage_hidden1_wgrad
         ctx.stash, ctx.upstream = stash, upstream
         if stash is not None:
-            # what the next layer's aggregation can be recomputed from (aggregate_hidden1)
+            # what the next layer's aggregation can be recomputed from (aggregate_hidden1).  The output
+            # without its place in the graph: ctx holds the stash, and an output that holds ctx in turn
+            # keeps graph and activations alive (until the collector runs, and past it in a capture)
             stash.update(agg=agg, x=x, w_l=w_l, b_l=b_l, w_r=w_r, sign=sign, epilogue=epilogue, p=p,
-                         out=out if epilogue == _lib.EPI_RELU_DROPOUT else None,
+                         out=out.detach() if epilogue == _lib.EPI_RELU_DROPOUT else None,
                          u=u_box.get("u") if u_box is not None else None,
                          weights_only=want_sign)
         return out
