@@ -40,6 +40,7 @@ def vector_width(f: int) -> int:
 
 _M64 = (1 << 64) - 1
 INPUT_SLOT = 63       # mix_seed's layer number of the input features' dropout
+DEPTH_DEFAULTS = {"norm": None, "residual": False, "input_dropout": 0.0}
 
 
 def mix_seed(base: int, step: int, layer: int = 0) -> int:
@@ -114,11 +115,6 @@ class SAGEConv(nn.Module):
 class GraphSAGE(nn.Module):
     """GraphSAGE encoder (reference ``GraphSAGE``, ``src/model/graphsage.py:33-157``)."""
 
-    # (of models pickled whole before these existed)
-    norm: Optional[str] = None
-    residual = False
-    input_dropout = 0.0
-
     def __init__(self, in_channels: int = 7, hidden_channels: int = 64, out_channels: int = 64,
                  num_layers: int = 2, dropout: float = 0.3, aggregator: str = "mean",
                  normalize_output: bool = True, cache_input_aggregation: bool = False,
@@ -166,6 +162,13 @@ class GraphSAGE(nn.Module):
         # processes did with torch's generators.  None: one draw from the CPU generator per layer.
         self._dropout_stream: Optional[tuple] = None
 
+    def __getattr__(self, name: str):
+        # models pickled whole before the depth options existed (attributes of the class would hide a module that a class
+        # made from this one keeps under such a name)
+        if name in DEPTH_DEFAULTS and name not in self.__dict__.get("_modules", ()):
+            return DEPTH_DEFAULTS[name]
+        return super().__getattr__(name)
+
     def set_dropout_stream(self, base_seed: Optional[int], step: int = 0) -> None:
         """Seed the dropout masks of the next training-mode forward from ``(base_seed, step,
         layer)`` instead of torch's CPU generator; ``None`` goes back to the generator."""
@@ -192,10 +195,11 @@ class GraphSAGE(nn.Module):
         graph = default_cache().get(edge_index, x.size(0))
         if dropout_seeds is not None and dropout_seeds.numel() != len(self.convs):
             raise ValueError(f"dropout_seeds must hold {len(self.convs)} seeds, got {tuple(dropout_seeds.shape)}")
-        dropped = self.training and self.input_dropout > 0.0
+        input_p = feature_dropout(self) if self.training else 0.0
+        dropped = input_p > 0.0
         if dropped:
-            x = dropout(x, self.input_dropout, seed=self._layer_seed(INPUT_SLOT, dropout_seeds, len(self.convs) - 1))
-        if self.norm is not None:
+            x = dropout(x, input_p, seed=self._layer_seed(INPUT_SLOT, dropout_seeds, len(self.convs) - 1))
+        if layer_normed(self):
             if keep_masks is not None:
                 raise ValueError("keep_masks are not taken with norm='layer': its masks are drawn in the kernel")
             return self._forward_normed(x, graph, dropout_seeds, not dropped)
@@ -347,16 +351,28 @@ class GraphSAGE(nn.Module):
     def reset_parameters(self) -> None:
         for conv in self.convs:
             conv.reset_parameters()
-        for norm in (self.norms if self.norm is not None else ()):
+        for norm in (self.norms if layer_normed(self) else ()):
             norm.reset_parameters()
 
     def count_parameters(self) -> int:
         return sum(p.numel() for p in self.parameters() if p.requires_grad)
 
 
+def layer_normed(model) -> bool:
+    """Whether the model is a GraphSAGE with ``norm="layer"``.  (A class made from it may keep a module of its own under
+    that name, and a model of another class whatever it likes.)"""
+    return isinstance(model, GraphSAGE) and model.norm == "layer"
+
+
+def feature_dropout(model) -> float:
+    """A GraphSAGE's ``input_dropout``; 0.0 where something else than a rate is kept under that name."""
+    p = model.input_dropout if isinstance(model, GraphSAGE) else 0.0
+    return float(p) if isinstance(p, (int, float)) and not isinstance(p, bool) else 0.0
+
+
 def depth_options(model_cfg: dict) -> dict:
     """The constructor's ``norm``, ``residual`` and ``input_dropout`` from a config's model section."""
-    return {k: model_cfg[k] for k in ("norm", "residual", "input_dropout") if k in model_cfg}
+    return {k: model_cfg[k] for k in DEPTH_DEFAULTS if k in model_cfg}
 
 
 def create_model(config: dict, device: Optional[torch.device] = None) -> GraphSAGE:

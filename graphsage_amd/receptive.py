@@ -53,7 +53,8 @@ def receptive_forward(model, x: torch.Tensor, graph: GraphCSR, targets: torch.Te
     remapped into T).  2-layer models only."""
     if len(model.convs) != 2:
         raise ValueError("the receptive-field step covers 2-layer models")
-    if model.norm is not None or model.input_dropout > 0.0:
+    from .graphsage import feature_dropout, layer_normed, vector_width
+    if layer_normed(model) or feature_dropout(model) > 0.0:
         raise ValueError("the receptive-field step covers models without norm and input_dropout")
     B = targets.numel()
     ids = torch.cat([targets, contexts, negatives.reshape(-1)])
@@ -68,7 +69,6 @@ def receptive_forward(model, x: torch.Tensor, graph: GraphCSR, targets: torch.Te
     # ---- layer 1 on the rows N1, sources read from the global feature table
     conv1, conv2 = model.convs[0], model.convs[1]
     w_l, w_r = conv1.lin_l.weight, conv1.lin_r.weight
-    from .graphsage import vector_width
     xg = x
     width = vector_width(x.size(1))
     if width != x.size(1):

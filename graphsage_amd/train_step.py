@@ -238,19 +238,20 @@ class TrainStep:
 
     def _graph_front(self, batch_size: int) -> None:
         """zero_grad -> forward -> loss on this rank's (static) batch -> backward -> stats."""
+        from .graphsage import feature_dropout, layer_normed
         model = self.model
         model.train()
         self.flat.zero_grad()
         masks = None
         p = float(getattr(model, "dropout_rate", 0.0))
-        normed = getattr(model, "norm", None) is not None
+        normed = layer_normed(model)
         if p > 0.0 and not normed:
             n = self.features.size(0)
             masks = [(torch.rand(n, conv.out_channels, device=self.features.device,
                                  generator=self._mask_gen) >= p).to(torch.uint8)
                      for conv in model.convs[:-1]]
         more = {}
-        if (normed and p > 0.0) or getattr(model, "input_dropout", 0.0) > 0.0:
+        if (normed and p > 0.0) or feature_dropout(model) > 0.0:
             # masks drawn in the kernels, from seeds that the graph rewrites on each replay
             more["dropout_seeds"] = torch.empty(len(model.convs), dtype=torch.int64,
                                                 device=self.features.device).random_(generator=self._mask_gen)
