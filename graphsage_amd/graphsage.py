@@ -371,8 +371,8 @@ def feature_dropout(model) -> float:
 
 
 def depth_options(model_cfg: dict) -> dict:
-    """The constructor's ``norm``, ``residual`` and ``input_dropout`` from a config's model section."""
-    return {k: model_cfg[k] for k in DEPTH_DEFAULTS if k in model_cfg}
+    """The constructor's ``norm``, ``residual`` and ``input_dropout`` from a config's model section (null: the default)."""
+    return {k: model_cfg[k] for k in DEPTH_DEFAULTS if model_cfg.get(k) is not None}
 
 
 def create_model(config: dict, device: Optional[torch.device] = None) -> GraphSAGE:

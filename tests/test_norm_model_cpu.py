@@ -35,3 +35,8 @@ def test_names_of_the_options_in_classes_made_from_the_model():
     other = torch.nn.Module()                   # a model that is no GraphSAGE
     other.norm, other.input_dropout = "layer", 0.5
     assert not layer_normed(other) and feature_dropout(other) == 0.0 and not layer_normed(torch.nn.Module())
+
+
+def test_options_that_a_config_leaves_empty_are_the_defaults():
+    m = create_model({"model": {"norm": None, "residual": None, "input_dropout": None}})
+    assert (m.norm, m.residual, m.input_dropout) == (None, False, 0.0)
