@@ -96,6 +96,7 @@ SIGNATURES = {
     "gsage_layer_norm_fwd": (C.c_int, [_p, _p, _p, _p, _i64, _i64, C.c_int, C.c_int, C.c_float, C.c_double,
                                        C.c_uint64, _p, _p, _p, _p, _p, _p]),
     "gsage_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, C.c_int]),
+    "gsage_layer_norm_bwd_joined_workspace_bytes": (_sz, [_i64, _i64, C.c_int]),
     "gsage_layer_norm_bwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, C.c_int, C.c_int, C.c_double,
                                        C.c_uint64, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "gsage_alias_build_host": (C.c_int, [_p, _i64, _p, _p]),

@@ -27,6 +27,7 @@ struct NormBwd {
   NormDrop d;
   void *gx, *gres, *gw, *gb;
   float *ws;
+  bool joined() const { return res || d.p > 0.f || gsum || gres; }
 };
 
 // Which kernel a row takes: K vectors of 16 bytes (V elements each) in each of R lanes of a wave, or of `row` threads of a
@@ -86,18 +87,20 @@ static inline int norm_blocks(int64_t M, int rows, int cap) {
 static inline bool norm_large(int64_t n, size_t size) { return n * (int64_t)size >= ((int64_t)256 << 20); }
 static inline bool norm_streams(int64_t M, int64_t F, size_t size) { return norm_large(M * F, size) && F * (int64_t)size % 128 == 0; }
 
-// Slabs of column sums that a backward call writes at most: for every NORM_FOLD_ROWS rows where streamed rows are short
-// (and 256 more, to which those are added up first), otherwise as few as keep the GPU busy
-constexpr int NORM_FOLD_ROWS = 32;
-static inline bool norm_folds(int64_t M, int64_t F, size_t size) {
-  return size == 4 && norm_streams(M, F, size) && F <= 128 && M <= (int64_t)1 << 27;      // (its launch's threads fit 32 bits)
+// Slabs of column sums that a backward call writes at most: one for every two turns of a workgroup where streamed rows are
+// short (and 256 more, to which those are added up first), otherwise as few as keep the GPU busy
+constexpr int NORM_FOLD_TURNS = 2, NORM_FOLD_THREADS = 512;
+static inline int norm_fold_rows(int64_t F) { return NORM_FOLD_TURNS * (NORM_FOLD_THREADS / norm_form(F, 4, true).row); }
+static inline bool norm_folds(int64_t M, int64_t F, size_t size, bool join) {
+  return !join && size == 4 && norm_streams(M, F, size) && F <= 128 && M <= (int64_t)1 << 27;      // (its launch's threads fit 32 bits)
 }
 static inline int norm_max_slabs(int64_t M, int64_t F) {
   const int64_t cap = F <= 512 ? 1024 : F <= 8192 ? 512 : 256;
   return (int)(M < cap ? M : cap);
 }
-static inline int64_t norm_ws_floats(int64_t M, int64_t F, size_t size) {
-  const int64_t few = norm_max_slabs(M, F), many = norm_folds(M, F, size) ? (M + NORM_FOLD_ROWS - 1) / NORM_FOLD_ROWS + 256 : 0;
+static inline int64_t norm_ws_floats(int64_t M, int64_t F, size_t size, bool join) {
+  const int64_t few = norm_max_slabs(M, F), rows = norm_folds(M, F, size, join) ? norm_fold_rows(F) : 0;
+  const int64_t many = rows ? (M + rows - 1) / rows + 256 : 0;
   return 2 * F * (many > few ? many : few > 0 ? few : 1);
 }
 

@@ -40,9 +40,13 @@ extern "C" int gsage_layer_norm_fwd(const void *x, const void *residual, const v
             gs_stream(stream));
 }
 
-extern "C" size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype) {
+static size_t ws_bytes_of(int64_t M, int64_t F, int dtype, bool join) {
   if (M < 0 || F <= 0 || F > MAX_F || M > MAX_N / F || bad_dtype(dtype)) return 0;
-  return gs_align_up((size_t)norm_ws_floats(M, F, dtype == GSAGE_F32 ? 4 : 2) * sizeof(float), 256);
+  return gs_align_up((size_t)norm_ws_floats(M, F, dtype == GSAGE_F32 ? 4 : 2, join) * sizeof(float), 256);
+}
+extern "C" size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype) { return ws_bytes_of(M, F, dtype, false); }
+extern "C" size_t gsage_layer_norm_bwd_joined_workspace_bytes(int64_t M, int64_t F, int dtype) {
+  return ws_bytes_of(M, F, dtype, true);
 }
 
 extern "C" int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, const void *x, const void *residual,
@@ -54,12 +58,12 @@ extern "C" int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, co
   if (wdtype != dtype && wdtype != GSAGE_F32) return GSAGE_ERR_INVALID_ARG;
   if (F > MAX_F || M > MAX_N / F) return GSAGE_ERR_UNSUPPORTED;
   if (M > 0 && (!grad_y || !x || !mean || !rstd)) return GSAGE_ERR_INVALID_ARG;
+  const NormBwd n{grad_y, grad_sum, x, residual, weight, mean, rstd, M, F, wdtype, drop_of(p, seed, seed_dev),
+                  grad_x, grad_residual, grad_weight, grad_bias, (float *)ws};
   if (grad_weight || grad_bias) {
     if (!ws) return GSAGE_ERR_INVALID_ARG;
-    if (ws_bytes < gsage_layer_norm_bwd_workspace_bytes(M, F, dtype)) return GSAGE_ERR_WORKSPACE;
+    if (ws_bytes < ws_bytes_of(M, F, dtype, n.joined())) return GSAGE_ERR_WORKSPACE;
   }
   const auto go = dtype == GSAGE_F32 ? norm_bwd_f32 : dtype == GSAGE_BF16 ? norm_bwd_bf16 : norm_bwd_f16;
-  return go(NormBwd{grad_y, grad_sum, x, residual, weight, mean, rstd, M, F, wdtype, drop_of(p, seed, seed_dev),
-                    grad_x, grad_residual, grad_weight, grad_bias, (float *)ws},
-            gs_stream(stream));
+  return go(n, gs_stream(stream));
 }

@@ -883,11 +883,12 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
   const int rows = ln_bwd_threads(TPR) / a.row, threads = rows * a.row, resident = ln_resident<kernel>(threads, lds);
   // Streamed fp32 tables of short rows in order, as the forward takes them, two turns a workgroup and a slab for each:
   // 10 M x 64 1.37 -> 1.25 ms, 4 M x 128 1.06 -> 1.01 (joined, and in 16 bits, nothing is gained: more arithmetic a byte).
-  // From 32 rows a slab on the slabs are 2 % of the traffic.
-  constexpr int turns = 2;
-  if (NT && !JOIN && d.ws && norm_folds(a.M, a.F, sizeof(T)) && rows * turns >= NORM_FOLD_ROWS) {
+  // A slab is written once and read once: 2 % of the traffic at its 64 rows of 64 columns, 4 % at 32 rows of 128.
+  constexpr int turns = NORM_FOLD_TURNS;
+  if (NT && !JOIN && d.ws && norm_folds(a.M, a.F, sizeof(T), JOIN)) {
     const int blocks = (int)((a.M + rows * turns - 1) / (rows * turns)), folded = norm_blocks(blocks, 1, 256);
     static_assert(!AHEAD || turns < ln_bwd_doubles(TPR, JOIN), "the column sums are fp32 words");
+    static_assert(TPR <= 0 || ln_bwd_threads(TPR) == NORM_FOLD_THREADS, "the workspace counts their rows a workgroup");
     // (room for two workgroups a compute unit: 1 M x 96 192 us, 218 with doubles')
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), few, st, a, Walk{0, (int64_t)rows * turns, rows, turns}, d);
     const int per = (blocks + folded - 1) / folded;
@@ -948,7 +949,7 @@ int ln_fwd(const NormFwd &n, hipStream_t st) {
 template <typename T>
 int ln_bwd(const NormBwd &n, hipStream_t st) {
   constexpr int V = Tab<T>::V;
-  const bool join = n.res || n.d.p > 0.f || n.gsum || n.gres, nt = norm_streams(n.M, n.F, sizeof(T));
+  const bool join = n.joined(), nt = norm_streams(n.M, n.F, sizeof(T));
   const NormForm f = norm_form(n.F, V, nt && !join);
   const Ln<T> a{(const T *)n.x, (const T *)n.res, n.w, nullptr, n.M, (int)n.F, n.wdtype, f.row, n.d};
   const Grads<T> d{(const T *)n.g, (const T *)n.gsum, n.mean, n.rstd, (T *)n.gx, (T *)n.gres,

@@ -64,7 +64,7 @@ def _rate(p: float) -> float:
     p = float(p)
     if not 0.0 <= p < 1.0 - 2.0 ** -25:           # (an fp32 number below 1)
         raise ValueError(f"dropout rate must be in [0, 1), got {p}")
-    return p
+    return p if p > 2.0 ** -150 else 0.0          # (what is 0 as an fp32 number drops nothing)
 
 
 def _seed(seed: Seed, device: torch.device) -> Union[int, torch.Tensor]:
@@ -144,7 +144,9 @@ def layer_norm_bwd(grad_y, grad_sum, x, residual, weight, stats, p: float, seed,
     gb = torch.empty(F, dtype=wdtype, device=dev) if need[3] else None
     ws, ws_bytes = None, 0
     if need[2] or need[3]:
-        ws_bytes = lib.gsage_layer_norm_bwd_workspace_bytes(M, F, code)
+        joined = residual is not None or grad_sum is not None or p > 0.0
+        ws_bytes = (lib.gsage_layer_norm_bwd_joined_workspace_bytes if joined
+                    else lib.gsage_layer_norm_bwd_workspace_bytes)(M, F, code)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     mean = stats.data_ptr()
     _call("layer_norm_bwd", dev, lib.gsage_layer_norm_bwd, grad_y.data_ptr(), _lib.ptr(grad_sum), x.data_ptr(),

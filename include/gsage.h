@@ -495,8 +495,9 @@ int gsage_skipgram_bwd_rows(const float *emb, int64_t N, int64_t D, const int64_
  *   grad_x, grad_residual [M,F] and grad_weight, grad_bias [F] (wdtype), each nullable.  x, residual,
  *   weight, p and seed as in the forward call, z and the mask are formed again.  Column sums go over
  *   per-workgroup slabs in slab order: bitwise reproducible.  M = 0: grad_weight = grad_bias = 0.
- *   ws: gsage_layer_norm_bwd_workspace_bytes(M, F, dtype) bytes (read only where grad_weight or
- *   grad_bias is wanted). */
+ *   ws: gsage_layer_norm_bwd_workspace_bytes(M, F, dtype) bytes (used only where grad_weight or
+ *   grad_bias is wanted); gsage_layer_norm_bwd_joined_workspace_bytes, never more, are enough with a
+ *   residual, grad_sum, grad_residual or p > 0 (10 M x 64 fp32: 80 MB, joined 0.5 MB). */
 enum gsage_dtype { GSAGE_F32 = 0, GSAGE_BF16 = 1, GSAGE_F16 = 2 };
 
 int gsage_dropout(const void *x, int64_t n, int dtype, double p, uint64_t seed,
@@ -506,6 +507,7 @@ int gsage_layer_norm_fwd(const void *x, const void *residual, const void *weight
                          uint64_t seed, const int64_t *seed_dev, void *y, void *sum, float *mean,
                          float *rstd, gsage_stream_t stream);
 size_t gsage_layer_norm_bwd_workspace_bytes(int64_t M, int64_t F, int dtype);
+size_t gsage_layer_norm_bwd_joined_workspace_bytes(int64_t M, int64_t F, int dtype);
 int gsage_layer_norm_bwd(const void *grad_y, const void *grad_sum, const void *x,
                          const void *residual, const void *weight, const float *mean,
                          const float *rstd, int64_t M, int64_t F, int dtype, int wdtype, double p,

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import graphsage_amd as gs
+from graphsage_amd import _lib
 
 import norm_reference as ref
 
@@ -92,3 +93,37 @@ def test_thousands_of_rows_a_thread_lose_no_bits(M, F, joined):
     y = gs.dropout_add_layer_norm(x, x if joined else None, None, b)
     gb, = torch.autograd.grad(y, b, torch.full((M, F), v, device="cuda"))
     assert float((gb.double() - M * v).abs().max()) <= 2.001 * U * M * v
+
+
+@pytest.mark.parametrize("M,F,dtype", [(1_050_011, 64, torch.float32), (524_301, 128, torch.float32), (700_001, 96, torch.float32),
+                                       (2_100_037, 32, torch.float32), (2_100_001, 64, torch.bfloat16), (33, 64, torch.float32),
+                                       (1, 20_000, torch.float32), (300_007, 1, torch.float16), (9000, 5000, torch.float16)])
+@pytest.mark.parametrize("joined", [False, True])
+def test_workspaces_are_large_enough_and_no_larger_than_said(M, F, dtype, joined):
+    """What a call is told to bring is enough (nothing behind it is written, less is refused), joined calls need no slab
+    for every few rows, and sums are the same whatever the workspace held."""
+    lib, code = _lib.load(), {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dtype]
+    size = (lib.gsage_layer_norm_bwd_joined_workspace_bytes if joined else lib.gsage_layer_norm_bwd_workspace_bytes)(M, F, code)
+    assert size <= lib.gsage_layer_norm_bwd_workspace_bytes(M, F, code)
+    if joined:
+        assert size <= max(1024 * 2 * F * 4, 256)
+    gen = torch.Generator(device="cuda").manual_seed(F)
+    x, g = (torch.empty(M, F, dtype=dtype, device="cuda").normal_(generator=gen) for _ in range(2))
+    res = torch.zeros_like(x) if joined else None
+    mean, rstd = x.float().mean(1), torch.ones(M, device="cuda")
+    st, outs = _lib.stream_handle(), []
+    for fill in (0x00, 0x7F):
+        ws = torch.full((size + 4096,), fill, dtype=torch.uint8, device="cuda")
+        gw, gb, gx = torch.empty(F, device="cuda"), torch.empty(F, device="cuda"), torch.empty_like(x)
+
+        def call(nbytes):
+            return lib.gsage_layer_norm_bwd(g.data_ptr(), None, x.data_ptr(), _lib.ptr(res), None, mean.data_ptr(),
+                                            rstd.data_ptr(), M, F, code, _lib.F32, 0.0, 0, None, gx.data_ptr(), None,
+                                            gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), nbytes, st)
+        assert call(size - 1) == -3
+        assert call(size) == 0
+        assert bool((ws[size:] == fill).all())
+        outs.append((gw, gb))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    gbd, size_b = g.double().sum(0), g.double().abs().sum(0)
+    assert bool(((outs[0][1].double() - gbd).abs() <= (66 + M / 64) * U * size_b).all())
