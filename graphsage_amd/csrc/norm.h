@@ -37,13 +37,14 @@ struct NormBwd {
 // Past a vector each of four lanes at least eight: a wave's accesses then take whole lines (4 M x 64 bf16 forward 0.167
 // ms, at four lanes x 2 0.220).  Two or four waves a row rather than three or five: eight fit a compute unit (40 000 x 1544
 // fp16 joined forward 79 us, 80); where that would be three or four waves of three vectors, nine to twelve of one (NORM_W1:
-// 8191 x 5120 bf16 joined with its sum forward 65 us, backward 112; in fours 66 and 122; 9000 x 2600 fp32 34 and 61, joined
-// 51 and 91; 36 and 62, 54 and 94).  Past 8192 columns (NORM_W) 16 elements a thread in up to sixteen waves, as many as a
+// of tables rotated past the caches 8191 x 5120 bf16 joined with its sum forward 65 us, backward 115; in fours 66 and 122;
+// 9000 x 2600 fp32 34 and 62, joined 51 and 90; 36 and 62, 54 and 94).  Past 8192 columns (NORM_W) 16 elements a thread in up to sixteen waves, as many as a
 // compute unit has room for: 8192 x 16000 bf16 forward 97 us, backward 176, joined 143 and 304; as eight waves with 32
 // elements a thread 103, 190, 174 and 367 (fp32 179, 288, 291, 661; 194, 315, 363, 956).  Large fp32 tables of whole cache
 // lines without residual or dropout stream best where neighbouring lanes hold neighbouring vectors (`stream`: 10 M x 64
-// forward 0.81 ms at 16 lanes x 1, 0.85 at 8 x 2, backward 1.25 and 1.34; 4 M x 128 0.65 and 0.68, 1.01 and 1.08; bf16
-// 2 M x 256 0.325 and 0.319, 0.548 and 0.541).
+// forward 0.81 ms at 16 lanes x 1, 0.85 at 8 x 2, backward 1.25 and 1.34; 4 M x 128 0.65 and 0.68, 1.01 and 1.08: 6.2 to
+// 6.4 TB/s; widths between, whose lanes do not all hold one vector, 6.1 at 3 M x 96, 5.9 at 2 M x 160, 5.6 to 5.9 at 192;
+// bf16 2 M x 256 0.325 and 0.319, 0.548 and 0.541).
 enum NormKind { NORM_ONE, NORM_R4, NORM_R8, NORM_R8x2, NORM_R8x3, NORM_R16, NORM_R16x2, NORM_R16x3, NORM_R32, NORM_R32x2,
                 NORM_R32x3, NORM_R64, NORM_R64x2, NORM_R64x3, NORM_B2, NORM_B3, NORM_B4, NORM_W1, NORM_W, NORM_LONG };
 struct NormForm { NormKind kind; int row; };      // threads of a row

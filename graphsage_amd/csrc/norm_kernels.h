@@ -417,8 +417,10 @@ constexpr int ln_bwd_doubles(int TPR, bool JOIN) { return TPR > 0 && JOIN ? 16 :
 
 // Workgroups of eight waves (fewer slabs than four would leave), or of the row's up to sixteen.  The row after is loaded a
 // row ahead where there are registers for it: not at 24 elements a thread (fp16 257 columns 39 us, joined 71; with four
-// waves that have them 42 and 83), nor at 16 of fp32 joined, nor at 16 in sixteen waves, which have 128 each; those read grad_sum, too, only when the weights are used up (fp32 8192 x 16000 joined 661 us; with the
-// other operands 758).
+// waves that have them 42 and 83), nor at 16 of fp32 joined, nor at 16 in sixteen waves, which have 128 each and, joined,
+// keep some in scratch (fp32 156 bytes a lane, forward 68; 16-bit 16); those read grad_sum, too, only when the weights are
+// used up (fp32 8192 x 16000 joined 661 us; with the other operands 758).  The doubles of nine to twelve waves of 16-bit rows
+// leave room for one workgroup a compute unit, which is the better half: 8191 x 5120 bf16 59 us, as two 66.
 constexpr bool ln_bwd_ahead(int V, int TPR, int K, bool JOIN) {
   return (TPR >= 0 || K == 1) && K * V < 24 && !(JOIN && K * V == 16 && V == 4);
 }
@@ -897,7 +899,11 @@ int ln_bwd_go(const Ln<T> &a, const Grads<T> &d, hipStream_t st) {
     hipLaunchKernelGGL(ln_slabs_k, dim3((unsigned)((2 * a.F + 15) / 16)), dim3(1024), 0, st, out, folded, a.F, a.wdtype, d.gw, d.gb);
     return 0;
   }
-  // (of the large tables sixteen waves a compute unit keep the memory busy; 24 of them were slower: 1 M x 256 fp32 0.56 against 0.52 ms)
+  // Of the large tables sixteen waves a compute unit keep the memory busy where a lane holds one vector, or two of a plain
+  // fp32 row; 24 of them were slower (1 M x 256 fp32 0.56 against 0.52 ms).  Joined rows of two vectors, plain ones of two in
+  // 16 bits and all of three run eight: registers (129 and more; of plain fp32 rows the doubles in LDS) allow no more.
+  // Sixteen of the joined fp32 ones, from a build that needed 115 registers, were slower: 1 M x 128 478 us against 433,
+  // 1 M x 256 965 against 905.
   const int most = norm_max_slabs(a.M, a.F), held = NT && resident > 512 ? 512 : resident;
   const int slabs = norm_blocks(a.M, rows, held < most ? held : most);
   const int64_t step = (int64_t)slabs * rows;

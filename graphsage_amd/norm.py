@@ -7,7 +7,8 @@ rounded once.  ``GraphSAGE(norm="layer")`` runs its hidden layers through them; 
 
 Dropout masks are those of the projection kernels: element ``i`` (row-major) is kept or not by a counter hash of
 ``(seed, i)`` alone (host mirror: :func:`graphsage_amd.rng.dropout_keep_mask`), so a mask is never stored and the
-backward draws it again.  A dropped element gives exactly 0, forward and backward, whatever it holds.
+backward draws it again.  Of tables below 2^32 elements the seed's two 32-bit halves count by their xor alone: 2^32 masks
+in all, seeds 1 and 2^32 the same one.  A dropped element gives exactly 0, forward and backward, whatever it holds.
 ``seed`` is an int, a one-element int64 tensor on the device (read when the kernel runs: a captured graph that
 rewrites it draws other masks on each replay, where an int is frozen into the graph), or None: one draw from
 torch's CPU generator.

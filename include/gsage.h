@@ -479,7 +479,8 @@ int gsage_skipgram_bwd_rows(const float *emb, int64_t N, int64_t D, const int64_
  * is rounded once.
  *
  *   keep(i) : the mask of GSAGE_EPI_RELU_DROPOUT: a hash of (seed, row-major element index i), kept
- *             with probability 1 - p, 0 <= p < 1.  Never stored.  seed_dev (nullable): one int64 on
+ *             with probability 1 - p, 0 <= p < 1.  Never stored.  Below element 2^32 the seed counts as
+ *             the xor of its two 32-bit halves: seeds 1 and 2^32 draw the same mask there.  seed_dev (nullable): one int64 on
  *             the device that takes the place of `seed`, read when the kernel runs, so that a captured
  *             graph draws other masks on each replay.
  *
