@@ -3031,11 +3031,12 @@ static int project_bwd_impl(const float *grad_out, const float *out, const float
   // 1. dpre
   const float *dp = grad_out;
   const float inv_keep = epilogue == GSAGE_EPI_RELU_DROPOUT ? 1.0f / (1.0f - p) : 1.0f;
-  const bool smallk = 2 * Fi <= 16 && (Fo <= 64 || Fo % 64 == 0);
   const bool relu_epi = epilogue == GSAGE_EPI_RELU || epilogue == GSAGE_EPI_RELU_DROPOUT;
   // first layer in training: no input gradient wanted -> the ReLU derivative is applied
-  // inside the dW kernel and dpre is never materialised
-  const bool fuse_relu = smallk && relu_epi && !grad_agg && !grad_x;
+  // inside the dW kernel and dpre is never materialised, if one of the two kernels that apply it
+  // takes the call (odd addresses past 64 columns go to dw_generic_k, which does not)
+  const bool dw16 = force_generic == 0 && Fo % 64 == 0 && Fi <= 8 && ((((uintptr_t)grad_out | (uintptr_t)out) & 15) == 0);
+  const bool fuse_relu = (dw16 || (Fi <= 8 && Fo <= 64)) && relu_epi && !grad_agg && !grad_x;
   if (epilogue != GSAGE_EPI_NONE && !fuse_relu) {
     hipLaunchKernelGGL(epilogue_bwd_k, dim3(gs_grid(N, 4, 256 * 16)), dim3(256), 0, st, grad_out,
                        out, rnorm, N, fo, epilogue, inv_keep, dpre);
