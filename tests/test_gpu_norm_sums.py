@@ -127,3 +127,18 @@ def test_workspaces_are_large_enough_and_no_larger_than_said(M, F, dtype, joined
     assert all(torch.equal(a, b) for a, b in zip(*outs))
     gbd, size_b = g.double().sum(0), g.double().abs().sum(0)
     assert bool(((outs[0][1].double() - gbd).abs() <= (66 + M / 64) * U * size_b).all())
+
+
+@pytest.mark.parametrize("F,dtype,joined,rows", [
+    (20, torch.float32, False, 64), (64, torch.float32, True, 64), (60, torch.bfloat16, False, 64), (62, torch.bfloat16, True, 64),
+    (200, torch.float16, False, 32), (300, torch.float32, False, 16), (1000, torch.float32, False, 4), (1200, torch.float32, True, 4),
+    (2000, torch.bfloat16, False, 4), (2600, torch.float32, False, 1), (5120, torch.bfloat16, False, 1),
+    (5120, torch.float16, True, 1)])
+def test_every_row_counts_once_around_each_flush(F, dtype, joined, rows):
+    """As many rows as make a thread's number of them one less, as many and one more than the registers' sums are kept for:
+    16 or 32, twice that, for 256 and 512 workgroups of `rows` rows at once."""
+    for workgroups in (256, 512):
+        for turns in (15, 16, 17, 23, 31, 32, 33, 63, 64, 65, 97):
+            for M in (workgroups * rows * turns - 1, workgroups * rows * turns):
+                if M * F <= 1 << 28 and 3 * M < 1 << 24:
+                    _exact(M, F, dtype, joined, torch.float32)
